@@ -5,6 +5,6 @@ Mirrors the reference's Python surface for this one path — ``evodiff.pretraine
 (hand-written gfx950 kernels behind the C ABI of ``include/evodiff_hip.h``).  There is no CPU path:
 calling the model without the library or without a GPU raises.
 """
-from . import constants, utils, model, pretrained, generate  # noqa: F401
+from . import constants, utils, ops, model, pretrained, generate  # noqa: F401
 
-__all__ = ["constants", "utils", "model", "pretrained", "generate"]
+__all__ = ["constants", "utils", "ops", "model", "pretrained", "generate"]

@@ -9,6 +9,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("EVODIFF_AMD_LIB") or os.path.join(_HERE, "csrc", "libevodiff_hip.so")
 
 PREC_FP32, PREC_BF16 = 0, 1
+DT_FP32, DT_BF16, DT_FP16, DT_E4M3 = 0, 1, 2, 3
+TOP_K_MAX = 32
 K_EMBED, K_LNACT, K_GEMM1X1, K_CONV, K_FINAL, K_CONV_OTHER, K_COUNT = 0, 1, 2, 3, 4, 5, 6
 KIND_NAMES = ("embed", "ln_act", "gemm1x1", "conv", "final", "conv_other")
 OPTIONS = {"prune": 0, "min_tuned_tiles": 1, "split_target": 2, "incremental": 3, "fuse_reduce_ln": 4,
@@ -19,7 +21,9 @@ OPTIONS = {"prune": 0, "min_tuned_tiles": 1, "split_target": 2, "incremental": 3
 SYMBOLS = ("ed_abi_version", "ed_last_error", "ed_model_create", "ed_model_destroy", "ed_model_load_tensor",
            "ed_model_commit", "ed_model_num_params", "ed_forward", "ed_forward_collect", "ed_score_nll", "ed_ar_sample", "ed_oadm_sample",
            "ed_d3pm_sample", "ed_model_set_option", "ed_probe_config", "ed_probe_read", "ed_debug_gemm",
-           "ed_debug_ln_act", "ed_debug_set_stamp_buffer", "ed_debug_gemm_splitk_noalloc", "ed_model_check_errors", "ed_model_get_config", "ed_ar_sample_scaffold")
+           "ed_debug_ln_act", "ed_debug_set_stamp_buffer", "ed_debug_gemm_splitk_noalloc", "ed_model_check_errors", "ed_model_get_config", "ed_ar_sample_scaffold",
+           "ed_fp8_quantize_rows", "ed_fp8_quantize_weight", "ed_fp8_linear_workspace", "ed_fp8_linear",
+           "ed_token_logprobs_workspace", "ed_token_logprobs", "ed_token_logprobs_backward", "ed_score_tokens")
 
 
 class EdConfig(C.Structure):
@@ -75,6 +79,17 @@ def load():
     lib.ed_debug_set_stamp_buffer.argtypes = [vp, i64]
     lib.ed_model_set_option.argtypes = [vp, i32, i32]
     lib.ed_probe_read.argtypes = [vp, C.POINTER(EdProbeStat), vp]
+    lib.ed_fp8_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    lib.ed_fp8_quantize_weight.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    lib.ed_fp8_linear_workspace.argtypes = [i64, i64, i64, i32]
+    lib.ed_fp8_linear_workspace.restype = i64
+    lib.ed_fp8_linear.argtypes = [vp, i32, i64, vp, vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp]
+    lib.ed_token_logprobs_workspace.argtypes = [i64, i64, i32]
+    lib.ed_token_logprobs_workspace.restype = i64
+    lib.ed_token_logprobs.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.ed_token_logprobs_backward.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, vp, vp, i32, vp, vp, vp, vp, vp, vp,
+                                               vp, vp]
+    lib.ed_score_tokens.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp]
     if lib.ed_abi_version() != 1:
         raise EvoDiffHipError("libevodiff_hip.so ABI version mismatch")
     _lib = lib

@@ -2,6 +2,7 @@
 // workspace, per-step launch sequence, hipGraph capture/replay and the HIP-event probe.
 #include "../../include/evodiff_hip.h"
 #include "kernels.hpp"
+#include "ops.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -105,6 +106,7 @@ struct ed_model {
 
   // workspace
   int ws_B = 0, ws_L = 0, ws_prec = -1;
+  DevBuf score_logits, score_ws;  // ed_score_tokens
   DevBuf X, X2, Abuf, Ybuf, Cpad, Cprune, state, tok, order, uni, qbuf, tvec;
   // Incremental leading layers (OA-DM, ED_OPT_INCREMENTAL): between two steps ONE token per sequence changes, so
   // layer k only changes within r_k = r_{k-1} + 2 d_k positions of it.  The first n_inc layers keep their outputs
@@ -1556,6 +1558,161 @@ int ed_probe_read(ed_model* m, ed_probe_stat* stats, void* stream) {
     m->event_pool.push_back({p.a, p.b});
   }
   m->pending.clear();
+  return ED_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// model-free operators
+// ------------------------------------------------------------------------------------------------
+namespace {
+
+bool plain_dtype(int dt) { return dt == ED_DT_FP32 || dt == ED_DT_BF16 || dt == ED_DT_FP16; }
+bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+constexpr int64_t MAX_DIM = 1LL << 30;     // rows, columns and classes each stay below this
+constexpr int64_t MAX_BLOCKS = 1LL << 28;  // 128-value blocks (or tiles) of one operand
+
+int check_values(const char* what, const void* p, int dt, int64_t row_stride, int64_t rows, int64_t K) {
+  if (!plain_dtype(dt)) return fail(ED_EINVAL, "%s: dtype must be fp32, bf16 or fp16 (got %d)", what, dt);
+  if (rows < 0 || rows >= MAX_DIM || K < 1 || K >= MAX_DIM || fp8_blocks(K) * rows >= MAX_BLOCKS)
+    return fail(ED_EINVAL, "%s: %lld x %lld values are out of range", what, (long long)rows, (long long)K);
+  if (row_stride < 0) return fail(ED_EINVAL, "%s: negative row stride", what);
+  if (rows > 0 && !p) return fail(ED_EINVAL, "%s: null pointer", what);
+  if (misaligned(p, (size_t)dt_bytes(dt))) return fail(ED_EINVAL, "%s: not aligned to its element", what);
+  return ED_OK;
+}
+
+int check_logits(const void* logits, int dt, int64_t row_stride, int64_t inner, int64_t outer_stride, int64_t rows,
+                 int64_t n, int top_k) {
+  if (!plain_dtype(dt)) return fail(ED_EINVAL, "logits: dtype must be fp32, bf16 or fp16 (got %d)", dt);
+  if (rows < 0 || rows >= MAX_DIM || n < 1 || n >= MAX_DIM)
+    return fail(ED_EINVAL, "logits: %lld rows of %lld classes are out of range", (long long)rows, (long long)n);
+  if (row_stride < 0 || outer_stride < 0 || inner < 1 || inner >= MAX_DIM)
+    return fail(ED_EINVAL, "logits: strides must not be negative and inner_rows must be in [1, 2^30)");
+  if (top_k < 0 || top_k > ED_TOP_K_MAX || top_k > n)
+    return fail(ED_EINVAL, "top_k = %d must be in [0, min(n_classes, %d)]", top_k, ED_TOP_K_MAX);
+  if (rows > 0 && !logits) return fail(ED_EINVAL, "null logits pointer");
+  if (misaligned(logits, (size_t)dt_bytes(dt))) return fail(ED_EINVAL, "logits: not aligned to their element");
+  return ED_OK;
+}
+
+}  // namespace
+
+int ed_fp8_quantize_rows(const void* x_dev, int x_dtype, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q_dev,
+                         uint8_t* scale_dev, void* stream) {
+  if (int rc = check_values("x", x_dev, x_dtype, row_stride, rows, K)) return rc;
+  if (rows == 0) return ED_OK;
+  if (!q_dev || !scale_dev) return fail(ED_EINVAL, "null q/scale pointer");
+  if (misaligned(q_dev, 16)) return fail(ED_EINVAL, "q_dev must be aligned to 16 bytes");
+  LAUNCH_TRY(launch_fp8_quantize_rows(x_dev, x_dtype, row_stride, rows, K, q_dev, scale_dev, (hipStream_t)stream));
+  return ED_OK;
+}
+
+int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, int64_t N, int64_t K, uint8_t* q_dev,
+                           uint8_t* scale_dev, void* stream) {
+  if (int rc = check_values("weight", w_dev, w_dtype, row_stride, N, K)) return rc;
+  if (N == 0) return ED_OK;
+  if (!q_dev || !scale_dev) return fail(ED_EINVAL, "null q/scale pointer");
+  if (misaligned(q_dev, 16)) return fail(ED_EINVAL, "q_dev must be aligned to 16 bytes");
+  LAUNCH_TRY(launch_fp8_quantize_weight(w_dev, w_dtype, row_stride, N, K, q_dev, scale_dev, (hipStream_t)stream));
+  return ED_OK;
+}
+
+int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype) {
+  if (M < 1 || N < 1 || K < 1 || M >= MAX_DIM || N >= MAX_DIM || K >= MAX_DIM) return 0;
+  return fp8_linear_workspace(M, N, K, x_dtype == ED_DT_E4M3);
+}
+
+int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
+                  const uint8_t* weight_scale_dev, const float* bias_dev, void* out_dev, int out_dtype, int64_t M, int64_t N,
+                  int64_t K, void* workspace_dev, int64_t workspace_bytes, void* stream) {
+  const bool quantised = x_dtype == ED_DT_E4M3;
+  if (quantised) {
+    if (M < 0 || M >= MAX_DIM || K < 1 || K >= MAX_DIM || fp8_blocks(K) * M >= MAX_BLOCKS)
+      return fail(ED_EINVAL, "x: %lld x %lld values are out of range", (long long)M, (long long)K);
+    if (row_stride != fp8_blocks(K) * FP8_BLOCK) return fail(ED_EINVAL, "quantised rows are ceil(K / 128) * 128 bytes apart");
+    if (misaligned(x_dev, 16)) return fail(ED_EINVAL, "quantised rows must be aligned to 16 bytes");
+  } else if (int rc = check_values("x", x_dev, x_dtype, row_stride, M, K)) {
+    return rc;
+  }
+  if (!plain_dtype(out_dtype)) return fail(ED_EINVAL, "out: dtype must be fp32, bf16 or fp16 (got %d)", out_dtype);
+  if (N < 1 || N >= MAX_DIM || fp8_blocks(K) * N >= MAX_BLOCKS) return fail(ED_EINVAL, "weight: %lld x %lld values are out of range", (long long)N, (long long)K);
+  if (((M + 15) / 16) * ((N + 15) / 16) >= MAX_BLOCKS) return fail(ED_EINVAL, "out: %lld x %lld values are out of range", (long long)M, (long long)N);
+  if (M == 0) return ED_OK;
+  if (!x_dev || (quantised && !x_scale_dev) || !weight_dev || !weight_scale_dev || !out_dev)
+    return fail(ED_EINVAL, "null x/scale/weight/out pointer");
+  if (misaligned(weight_dev, 16)) return fail(ED_EINVAL, "the weight must be aligned to 16 bytes");
+  if (misaligned(out_dev, (size_t)dt_bytes(out_dtype)) || misaligned(bias_dev, 4)) return fail(ED_EINVAL, "out/bias: not aligned to their element");
+  const int64_t need = fp8_linear_workspace(M, N, K, quantised);
+  if (need > 0 && (!workspace_dev || workspace_bytes < need || misaligned(workspace_dev, 16)))
+    return fail(ED_EINVAL, "workspace: %lld bytes at a 16-byte boundary are needed (ed_fp8_linear_workspace)", (long long)need);
+  const Fp8Linear p{x_dev, x_dtype, row_stride, x_scale_dev, weight_dev, weight_scale_dev, bias_dev, out_dev, out_dtype,
+                    M, N, K, workspace_dev};
+  LAUNCH_TRY(launch_fp8_linear(p, (hipStream_t)stream));
+  return ED_OK;
+}
+
+int64_t ed_token_logprobs_workspace(int64_t rows, int64_t n_classes, int top_k) {
+  if (rows < 1 || n_classes < 1 || rows >= MAX_DIM || n_classes >= MAX_DIM || top_k < 0 || top_k > ED_TOP_K_MAX) return 0;
+  return token_logprobs_workspace(rows, n_classes, top_k);
+}
+
+int ed_token_logprobs(const void* logits_dev, int dtype, int64_t row_stride, int64_t inner_rows, int64_t outer_stride,
+                      int64_t rows, int64_t n_classes, const int64_t* targets_dev, const uint8_t* select_dev, int top_k,
+                      float* logprob_dev, float* entropy_dev, float* row_stats_dev, float* top_logprob_dev,
+                      int64_t* top_token_dev, void* workspace_dev, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_logits(logits_dev, dtype, row_stride, inner_rows, outer_stride, rows, n_classes, top_k)) return rc;
+  if (rows == 0) return ED_OK;
+  if (!entropy_dev || (targets_dev && !logprob_dev)) return fail(ED_EINVAL, "null logprob/entropy pointer");
+  if (top_k > 0 && (!top_logprob_dev || !top_token_dev)) return fail(ED_EINVAL, "null top_logprob/top_token pointer");
+  const int64_t need = token_logprobs_workspace(rows, n_classes, top_k);
+  if (need > 0 && (!workspace_dev || workspace_bytes < need || misaligned(workspace_dev, 16)))
+    return fail(ED_EINVAL, "workspace: %lld bytes at a 16-byte boundary are needed (ed_token_logprobs_workspace)", (long long)need);
+  const LogitsView x{logits_dev, dtype, rows, inner_rows, row_stride, outer_stride, (int)n_classes};
+  const LogprobsOut out{logprob_dev, entropy_dev, row_stats_dev, top_logprob_dev, top_token_dev};
+  LAUNCH_TRY(launch_token_logprobs(x, targets_dev, select_dev, top_k, out, workspace_dev, (hipStream_t)stream));
+  return ED_OK;
+}
+
+int ed_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row_stride, int64_t inner_rows,
+                               int64_t outer_stride, int64_t rows, int64_t n_classes, int64_t columns,
+                               const int64_t* targets_dev, const uint8_t* select_dev, int top_k,
+                               const float* row_stats_dev, const float* entropy_dev, const int64_t* top_token_dev,
+                               const float* grad_logprob_dev, const float* grad_entropy_dev, const float* grad_top_dev,
+                               void* dlogits_dev, void* stream) {
+  if (int rc = check_logits(logits_dev, dtype, row_stride, inner_rows, outer_stride, rows, n_classes, top_k)) return rc;
+  if (columns < n_classes || columns >= MAX_DIM) return fail(ED_EINVAL, "columns must be in [n_classes, 2^30)");
+  if (rows == 0) return ED_OK;
+  if (!row_stats_dev || !entropy_dev || !dlogits_dev) return fail(ED_EINVAL, "null row_stats/entropy/dlogits pointer");
+  if (grad_logprob_dev && !targets_dev) return fail(ED_EINVAL, "a gradient of logprob needs the targets");
+  if (grad_top_dev && top_k > 0 && !top_token_dev) return fail(ED_EINVAL, "a gradient of top_logprob needs top_token");
+  if (misaligned(dlogits_dev, (size_t)dt_bytes(dtype))) return fail(ED_EINVAL, "dlogits: not aligned to their element");
+  const LogitsView x{logits_dev, dtype, rows, inner_rows, row_stride, outer_stride, (int)n_classes};
+  const LogprobsGrad g{row_stats_dev, entropy_dev, top_token_dev, grad_logprob_dev, grad_entropy_dev,
+                       top_k > 0 ? grad_top_dev : nullptr, dlogits_dev, columns};
+  LAUNCH_TRY(launch_token_logprobs_backward(x, targets_dev, select_dev, top_k, g, (hipStream_t)stream));
+  return ED_OK;
+}
+
+int ed_score_tokens(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_dev, const int64_t* targets_dev,
+                    const uint8_t* select_dev, int B, int L, int n_classes, int top_k, float* logprob_dev,
+                    float* entropy_dev, float* top_logprob_dev, int64_t* top_token_dev, int precision, void* stream) {
+  int rc = check_shape(m, B, L, precision);
+  if (rc) return rc;
+  if (!targets_dev || !logprob_dev || !entropy_dev) return fail(ED_EINVAL, "null targets/logprob/entropy pointer");
+  const int V = m->cfg.n_tokens;
+  if (n_classes < 1 || n_classes > V) return fail(ED_EINVAL, "n_classes must be in [1, n_tokens]");
+  if (top_k < 0 || top_k > n_classes || top_k > ED_TOP_K_MAX) return fail(ED_EINVAL, "top_k = %d must be in [0, min(n_classes, %d)]", top_k, ED_TOP_K_MAX);
+  if (top_k > 0 && (!top_logprob_dev || !top_token_dev)) return fail(ED_EINVAL, "null top_logprob/top_token pointer");
+  hipStream_t s = (hipStream_t)stream;
+  HIP_TRY(hipSetDevice(m->device));
+  const int64_t rows = (int64_t)B * L;
+  HIP_TRY(m->score_logits.ensure((size_t)rows * V * 4));
+  HIP_TRY(m->score_ws.ensure((size_t)token_logprobs_workspace(rows, n_classes, top_k)));
+  if ((rc = ed_forward(m, tokens_dev, timesteps_dev, B, L, m->score_logits.as<float>(), precision, stream))) return rc;
+  LAUNCH_TRY(launch_check_targets(targets_dev, select_dev, rows, n_classes, m->ln_err_dev, s));
+  const LogitsView x{m->score_logits.p, DT_FP32, rows, rows, V, 0, n_classes};
+  const LogprobsOut out{logprob_dev, entropy_dev, nullptr, top_logprob_dev, top_token_dev};
+  LAUNCH_TRY(launch_token_logprobs(x, targets_dev, select_dev, top_k, out, m->score_ws.p, s));
   return ED_OK;
 }
 

@@ -228,7 +228,7 @@ __device__ __forceinline__ float gelu_sigmoid_fit(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(w));
 }
 
-// two elements at a time: hipcc selects the packed fp32 instructions (v_pk_mul/fma/add_f32) for <2 x float>
+// two elements at a time (plain fp32 instructions: the packed ones are switched off in the Makefile)
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 gelu_sigmoid_fit2(f32x2 x) {
   constexpr float LOG2E = 1.4426950408889634f;

@@ -102,7 +102,7 @@ __device__ __forceinline__ unsigned ln_publish(const GemmProblem& g, Acc& acc, c
       red[(wr * 64 + ip * 16 + fr) * 8 + wc * 4 + fq] = lnf32x2{0.f, 1.f};
       continue;
     }
-    // one pass, two elements per instruction (v_pk_add_f32 / v_pk_fma_f32): sum and sum of squares of the lane's NL
+    // one pass, two elements at a time: sum and sum of squares of the lane's NL
     // values; M2 about the lane's own mean is q - s^2 / NL (a cancellation over NL = 32 / 40 values only: the merge
     // of the partials below is the stable form)
     lnf32x2 s2 = {0.f, 0.f}, q2 = {0.f, 0.f};

@@ -7,8 +7,11 @@
 #include "../../include/evodiff_hip.h"
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
+
+#include <tuple>
 
 namespace {
 
@@ -116,6 +119,208 @@ at::Tensor score_nll(int64_t handle, const at::Tensor& tokens, const at::Tensor&
   return nll;
 }
 
+// ---- model-free operators (evodiff_amd/ops.py documents them) ----
+int dtype_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "evodiff_amd: ", name, " must live on the GPU (there is no CPU path)");
+  if (t.scalar_type() == at::kFloat) return ED_DT_FP32;
+  if (t.scalar_type() == at::kBFloat16) return ED_DT_BF16;
+  TORCH_CHECK(t.scalar_type() == at::kHalf, "evodiff_amd: ", name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  return ED_DT_FP16;
+}
+
+void same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
+  TORCH_CHECK(a.device() == b.device(), "evodiff_amd: ", name, " must be on the device of the first operand");
+}
+
+template <typename T>
+T* ptr_or_null(const c10::optional<at::Tensor>& t) { return t.has_value() ? (T*)t->data_ptr() : nullptr; }
+
+int64_t blocks_of(int64_t k) { return (k + 127) / 128; }
+
+// (rows, K) with one row stride and contiguous columns; other layouts are copied
+at::Tensor as_rows(const at::Tensor& x, const char* name) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "evodiff_amd: ", name, " must have a non-empty last dimension");
+  at::Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor& x, bool square) {
+  const int dt = dtype_of(x, square ? "w" : "x");
+  TORCH_CHECK(!square || x.dim() == 2, "evodiff_amd: a weight must be (N, K)");
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor r = as_rows(x, square ? "w" : "x");
+  const int64_t rows = r.size(0), k = r.size(1), kb = blocks_of(k);
+  at::Tensor q = at::empty({rows, kb * 128}, x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty({square ? blocks_of(rows) : rows, kb}, x.options().dtype(at::kFloat8_e8m0fnu));
+  check((square ? ed_fp8_quantize_weight : ed_fp8_quantize_rows)(r.data_ptr(), dt, r.stride(0), rows, k, (uint8_t*)q.data_ptr(),
+                                                                 (uint8_t*)scale.data_ptr(), current_stream(x)));
+  return {q, scale};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor& x) { return quantize(x, false); }
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_weight(const at::Tensor& w) { return quantize(w, true); }
+
+at::Tensor linear_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& x_scale, const at::Tensor& weight,
+                      const at::Tensor& weight_scale, const c10::optional<at::Tensor>& bias,
+                      c10::optional<at::ScalarType> out_dtype) {
+  want(weight, at::kFloat8_e4m3fn, "weight.q");
+  want(weight_scale, at::kFloat8_e8m0fnu, "weight.scale");
+  same_device(weight, x, "x");
+  same_device(weight, weight_scale, "weight.scale");
+  TORCH_CHECK(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0 && weight.size(1) % 128 == 0, "evodiff_amd: weight.q must be (N, Kb * 128)");
+  const int64_t N = weight.size(0), kb = weight.size(1) / 128;
+  TORCH_CHECK(weight_scale.dim() == 2 && weight_scale.size(0) == blocks_of(N) && weight_scale.size(1) == kb,
+              "evodiff_amd: weight.scale must be (", blocks_of(N), ", ", kb, "), got ", weight_scale.sizes());
+  int dt = ED_DT_E4M3;
+  if (x_scale.has_value()) {
+    want(x, at::kFloat8_e4m3fn, "x.q");
+    want(*x_scale, at::kFloat8_e8m0fnu, "x.scale");
+    same_device(weight, *x_scale, "x.scale");
+    TORCH_CHECK(x.dim() == 2 && x_scale->dim() == 2 && x_scale->size(0) == x.size(0) && x_scale->size(1) * 128 == x.size(1),
+                "evodiff_amd: x.q must be (rows, Kb * 128) and x.scale (rows, Kb)");
+  } else {
+    dt = dtype_of(x, "x");
+  }
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && blocks_of(x.size(-1)) == kb, "evodiff_amd: x has ", x.dim() ? x.size(-1) : 0,
+              " channels, the weight is laid out for ", kb * 128 - 127, " to ", kb * 128);
+  if (bias.has_value()) {
+    want(*bias, at::kFloat, "bias");
+    same_device(weight, *bias, "bias");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "evodiff_amd: bias must be (", N, ")");
+  }
+  const at::ScalarType ot = out_dtype.has_value() ? *out_dtype : x_scale.has_value() ? at::kBFloat16 : x.scalar_type();
+  TORCH_CHECK(ot == at::kFloat || ot == at::kBFloat16 || ot == at::kHalf, "evodiff_amd: out_dtype must be float32, bfloat16 or float16, got ", ot);
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor r = as_rows(x, "x");
+  const int64_t M = r.size(0), K = r.size(1);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = N;
+  at::Tensor out = at::empty(shape, x.options().dtype(ot));
+  const int64_t need = ed_fp8_linear_workspace(M, N, K, dt);
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, x.options().dtype(at::kByte));
+  check(ed_fp8_linear(r.data_ptr(), dt, r.stride(0), ptr_or_null<uint8_t>(x_scale), (const uint8_t*)weight.data_ptr(),
+                      (const uint8_t*)weight_scale.data_ptr(), ptr_or_null<float>(bias), out.data_ptr(), dtype_of(out, "out"), M, N,
+                      K, need > 0 ? ws.data_ptr() : nullptr, need, current_stream(x)));
+  return out;
+}
+
+// Logits (..., V) as rows of one or two strides; others are copied.
+struct LogitRows {
+  at::Tensor t;
+  int64_t rows, row_stride, inner, outer_stride;
+};
+LogitRows logit_rows(const at::Tensor& logits) {
+  const int64_t V = logits.size(-1);
+  LogitRows r{logits, V > 0 ? logits.numel() / V : 0, V, 1, 0};
+  if (r.rows == 0) return r;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    r.t = attempt == 0 ? logits : logits.contiguous();
+    if (V > 1 && r.t.stride(-1) != 1) continue;
+    std::vector<std::pair<int64_t, int64_t>> lead;  // (size, stride), innermost first, neighbours joined where they are one run
+    for (int64_t d = r.t.dim() - 2; d >= 0; --d) {
+      const int64_t n = r.t.size(d), st = r.t.stride(d);
+      if (n == 1) continue;
+      if (!lead.empty() && st == lead.back().first * lead.back().second) lead.back().first *= n;
+      else lead.push_back({n, st});
+    }
+    if (lead.size() > 2) continue;
+    r.inner = lead.empty() ? 1 : lead[0].first;
+    r.row_stride = lead.empty() ? V : lead[0].second;
+    r.outer_stride = lead.size() > 1 ? lead[1].second : 0;
+    return r;
+  }
+  return r;  // (a contiguous tensor always returns above)
+}
+
+void check_row_tensor(const c10::optional<at::Tensor>& t, const at::Tensor& logits, const char* name) {
+  if (!t.has_value()) return;
+  TORCH_CHECK(t->is_cuda(), "evodiff_amd: ", name, " must live on the GPU (there is no CPU path)");
+  same_device(logits, *t, name);
+  TORCH_CHECK(t->sizes() == logits.sizes().slice(0, logits.dim() - 1), "evodiff_amd: ", name, " must be shaped like the logits without classes, got ", t->sizes());
+}
+
+struct RowInputs {  // targets and select as the library reads them
+  c10::optional<at::Tensor> targets, select;
+};
+RowInputs row_inputs(const at::Tensor& logits, const c10::optional<at::Tensor>& targets, const c10::optional<at::Tensor>& select) {
+  RowInputs r;
+  check_row_tensor(targets, logits, "targets");
+  check_row_tensor(select, logits, "select");
+  if (targets.has_value()) {
+    TORCH_CHECK(targets->scalar_type() == at::kLong || targets->scalar_type() == at::kInt, "evodiff_amd: targets must be int64 or int32, got ", targets->scalar_type());
+    r.targets = targets->to(at::kLong).contiguous();
+  }
+  if (select.has_value()) {
+    TORCH_CHECK(select->scalar_type() == at::kBool || select->scalar_type() == at::kByte, "evodiff_amd: select must be bool or uint8, got ", select->scalar_type());
+    r.select = select->contiguous();
+  }
+  return r;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
+    const at::Tensor& logits, const c10::optional<at::Tensor>& targets, const c10::optional<at::Tensor>& select, int64_t top_k,
+    int64_t n_classes, bool with_stats) {
+  const int dt = dtype_of(logits, "logits");
+  TORCH_CHECK(logits.dim() >= 1 && n_classes >= 1 && n_classes <= logits.size(-1), "evodiff_amd: n_classes must be in [1, ", logits.dim() ? logits.size(-1) : 0, "], got ", n_classes);
+  TORCH_CHECK(top_k >= 0 && top_k <= n_classes && top_k <= ED_TOP_K_MAX, "evodiff_amd: top_k must be in [0, min(n_classes, ", ED_TOP_K_MAX, ")], got ", top_k);
+  const c10::DeviceGuard guard(logits.device());
+  const RowInputs in = row_inputs(logits, targets, select);
+  const LogitRows r = logit_rows(logits);
+  std::vector<int64_t> shape = logits.sizes().vec();
+  shape.pop_back();
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor logprob = targets.has_value() ? at::empty(shape, f32) : at::empty({0}, f32);
+  at::Tensor entropy = at::empty(shape, f32);
+  at::Tensor stats = at::empty({with_stats ? r.rows : 0, 2}, f32);
+  shape.push_back(top_k);
+  at::Tensor top = at::empty(shape, f32), token = at::empty(shape, f32.dtype(at::kLong));
+  const int64_t need = ed_token_logprobs_workspace(r.rows, n_classes, (int)top_k);
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, f32.dtype(at::kByte));
+  check(ed_token_logprobs(r.t.data_ptr(), dt, r.row_stride, r.inner, r.outer_stride, r.rows, n_classes, ptr_or_null<int64_t>(in.targets),
+                          ptr_or_null<uint8_t>(in.select), (int)top_k, targets.has_value() ? logprob.data_ptr<float>() : nullptr,
+                          entropy.data_ptr<float>(), with_stats ? stats.data_ptr<float>() : nullptr, top.data_ptr<float>(),
+                          token.data_ptr<int64_t>(), need > 0 ? ws.data_ptr() : nullptr, need, current_stream(logits)));
+  return {logprob, entropy, top, token, stats};
+}
+
+at::Tensor token_logprobs_backward(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
+                                   const c10::optional<at::Tensor>& select, int64_t top_k, int64_t n_classes,
+                                   const at::Tensor& stats, const at::Tensor& entropy, const at::Tensor& top_token,
+                                   const c10::optional<at::Tensor>& g_logprob, const c10::optional<at::Tensor>& g_entropy,
+                                   const c10::optional<at::Tensor>& g_top) {
+  const int dt = dtype_of(logits, "logits");
+  TORCH_CHECK(logits.dim() >= 1 && n_classes >= 1 && n_classes <= logits.size(-1), "evodiff_amd: n_classes must be in [1, V]");
+  TORCH_CHECK(top_k >= 0 && top_k <= n_classes && top_k <= ED_TOP_K_MAX, "evodiff_amd: top_k out of range");
+  const c10::DeviceGuard guard(logits.device());
+  const RowInputs in = row_inputs(logits, targets, select);
+  const LogitRows r = logit_rows(logits);
+  want(stats, at::kFloat, "row_stats");
+  want(entropy, at::kFloat, "entropy");
+  want(top_token, at::kLong, "top_token");
+  same_device(logits, stats, "row_stats");
+  same_device(logits, entropy, "entropy");
+  same_device(logits, top_token, "top_token");
+  TORCH_CHECK(stats.numel() == 2 * r.rows && entropy.numel() == r.rows && top_token.numel() == r.rows * top_k, "evodiff_amd: row_stats, entropy and top_token must be those of the forward call");
+  c10::optional<at::Tensor> g[3];
+  const c10::optional<at::Tensor>* given[3] = {&g_logprob, &g_entropy, &g_top};
+  for (int i = 0; i < 3; ++i)
+    if (given[i]->has_value()) {
+      const at::Tensor& t = **given[i];
+      TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.numel() == r.rows * (i == 2 ? top_k : 1), "evodiff_amd: gradients must be fp32 of the outputs' shapes");
+      same_device(logits, t, "a gradient");
+      g[i] = t.contiguous();
+    }
+  at::Tensor grad = at::empty(logits.sizes(), logits.options());
+  check(ed_token_logprobs_backward(r.t.data_ptr(), dt, r.row_stride, r.inner, r.outer_stride, r.rows, n_classes, logits.size(-1),
+                                   ptr_or_null<int64_t>(in.targets), ptr_or_null<uint8_t>(in.select), (int)top_k,
+                                   stats.data_ptr<float>(), entropy.data_ptr<float>(), top_token.data_ptr<int64_t>(),
+                                   ptr_or_null<float>(g[0]), ptr_or_null<float>(g[1]), ptr_or_null<float>(g[2]), grad.data_ptr(),
+                                   current_stream(logits)));
+  return grad;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(evodiff_amd, m) {
@@ -123,6 +328,11 @@ TORCH_LIBRARY(evodiff_amd, m) {
   m.def("oadm_sample_(int handle, Tensor(a!) tokens, Tensor order, Tensor uniforms, int n_draw, int precision, bool use_graph) -> Tensor(a!)");
   m.def("d3pm_sample_(int handle, Tensor(a!) tokens, Tensor Q, Tensor Qbar, Tensor uniforms, int K, int t_start, int n_steps, int precision, bool use_graph) -> Tensor(a!)");
   m.def("score_nll(int handle, Tensor tokens, Tensor timesteps, Tensor targets, Tensor? select, int n_classes, int precision) -> Tensor");
+  m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)");
+  m.def("quantize_fp8_weight(Tensor w) -> (Tensor, Tensor)");
+  m.def("linear_fp8(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType? out_dtype) -> Tensor");
+  m.def("token_logprobs(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes, bool with_stats) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("token_logprobs_backward(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes, Tensor row_stats, Tensor entropy, Tensor top_token, Tensor? grad_logprob, Tensor? grad_entropy, Tensor? grad_top) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(evodiff_amd, CUDA, m) {
@@ -130,4 +340,9 @@ TORCH_LIBRARY_IMPL(evodiff_amd, CUDA, m) {
   m.impl("oadm_sample_", &oadm_sample_);
   m.impl("d3pm_sample_", &d3pm_sample_);
   m.impl("score_nll", &score_nll);
+  m.impl("quantize_fp8", &quantize_fp8);
+  m.impl("quantize_fp8_weight", &quantize_fp8_weight);
+  m.impl("linear_fp8", &linear_fp8);
+  m.impl("token_logprobs", &token_logprobs);
+  m.impl("token_logprobs_backward", &token_logprobs_backward);
 }

@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .ops import TokenLogprobs
 
 
 class _ParamOnly(nn.Module):
@@ -277,6 +278,48 @@ class ByteNetLMTime(nn.Module):
                                         sel.data_ptr() if sel is not None else None, B, L, n_classes, nll.data_ptr(),
                                         self._prec(), stream))
         return nll
+
+    def score_tokens(self, x, y, targets, select=None, n_classes=None, top_k=0, validate=True):
+        """Forward + what the model says about ``targets`` at every position, on the GPU: an ``ops.TokenLogprobs`` of (B, L)
+        ``logprob`` and ``entropy`` (fp32, nats, over the first ``n_classes`` classes) and the ``top_k`` likeliest tokens
+        (B, L, top_k) with their log probabilities.  ``logprob`` is minus what ``score_nll`` returns; positions where ``select``
+        (B, L) is false hold 0, their tokens -1."""
+        if not x.is_cuda:
+            raise _lib.EvoDiffHipError("evodiff_amd has no CPU path: move the inputs to the GPU")
+        if x.dim() != 2:
+            raise ValueError("x must be (batch, length)")
+        B, L = x.shape
+        n_classes = self.hparams["n_tokens"] if n_classes is None else int(n_classes)
+        top_k = int(top_k)
+        if not 1 <= n_classes <= self.hparams["n_tokens"]:
+            raise ValueError("n_classes must be in [1, n_tokens=%d]" % self.hparams["n_tokens"])
+        if not 0 <= top_k <= min(n_classes, _lib.TOP_K_MAX):
+            raise ValueError("top_k must be in [0, min(n_classes, %d)]" % _lib.TOP_K_MAX)
+        handle = self.hip_handle(x.device)
+        lib = _lib.load()
+        x = x.to(torch.long).contiguous()
+        y = y.to(device=x.device, dtype=torch.long).contiguous()
+        if self.hparams["timesteps"] > 0 and y.numel() != B:
+            raise IndexError("y must hold one timestep in [0, timesteps) per sequence")
+        targets = targets.to(device=x.device, dtype=torch.long).contiguous()
+        if targets.shape != x.shape:
+            raise ValueError("targets must have the shape of x")
+        sel = None
+        if select is not None:
+            sel = select.to(device=x.device).reshape(B, L).ne(0).to(torch.uint8).contiguous()
+        if validate:
+            self._check_ranges(x, y, targets, sel, n_classes)
+        logprob = torch.empty((B, L), dtype=torch.float32, device=x.device)
+        entropy = torch.empty_like(logprob)
+        top_logprob = torch.empty((B, L, top_k), dtype=torch.float32, device=x.device)
+        top_token = torch.empty((B, L, top_k), dtype=torch.long, device=x.device)
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        with torch.cuda.device(x.device):
+            _lib.check(lib.ed_score_tokens(handle, x.data_ptr(), y.data_ptr(), targets.data_ptr(),
+                                           sel.data_ptr() if sel is not None else None, B, L, n_classes, top_k,
+                                           logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr(),
+                                           top_token.data_ptr(), self._prec(), stream))
+        return TokenLogprobs(logprob, entropy, top_logprob, top_token)
 
     # ------------------------------------------------------------------ fused sampling loops (C ABI)
     def oadm_sample(self, sample, order, uniforms, n_draw, return_probs=False):

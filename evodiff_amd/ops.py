@@ -1,0 +1,121 @@
+"""Operators for programs that score or generate with hidden states and logits of their own (no model handle):
+
+* ``token_logprobs`` - the log probability of given tokens with the entropy and the top alternatives of every row, with its
+  gradient to the logits; ``ByteNetLMTime.score_tokens`` runs it behind the model's own forward;
+* ``quantize_fp8`` / ``quantize_fp8_weight`` / ``linear_fp8`` - 8-bit floating point with a power-of-two scale for each block
+  of 128, and the product on it.
+
+They run on PyTorch's current stream of the tensors' device, through ``torch.ops.evodiff_amd`` (csrc/torch_ops.cpp) over the
+C ABI (``ed_token_logprobs``, ``ed_fp8_*`` in include/evodiff_hip.h).  There is no CPU path.  Outputs and workspaces come from
+PyTorch's allocator, so the calls can be captured into a HIP graph.  A backward pass that is captured should ask for its
+gradients with ``torch.autograd.grad``: ``.backward()`` accumulates into leaves on the stream that first used them.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import torch_ops
+from ._lib import EvoDiffHipError
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: ``q`` (rows, Kb * 128) float8_e4m3fn, ``scale`` (rows, Kb) float8_e8m0fnu, Kb = ceil(K / 128)."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+class Fp8Weight(NamedTuple):
+    """A weight in 8 bits: ``q`` (N, Kb * 128) float8_e4m3fn, ``scale`` (ceil(N / 128), Kb) float8_e8m0fnu."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row of the logits: ``logprob`` of the given token (None without targets), ``entropy`` in nats, and the ``top_k``
+    likeliest tokens ``top_token`` (int64) with their ``top_logprob``.  fp32, shaped like the logits without classes."""
+    logprob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor
+    top_token: torch.Tensor
+
+
+def _on_gpu(*tensors):
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise EvoDiffHipError("evodiff_amd has no CPU path: move the inputs to the GPU")
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError("all tensors of a call must be on one device")
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """``x`` (..., K) fp32 / bf16 / fp16 -> rows in 8 bits, a scale for 128 channels of a row (leading dimensions are
+    flattened).  Rounded to nearest even; infinities and NaN become NaN."""
+    _on_gpu(x)
+    return Fp8Rows(*torch_ops.load().quantize_fp8(x.detach()))
+
+
+def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
+    """``w`` (N, K) fp32 / bf16 / fp16 -> a weight in 8 bits, one scale for 128 x 128 values."""
+    _on_gpu(w)
+    return Fp8Weight(*torch_ops.load().quantize_fp8_weight(w.detach()))
+
+
+def linear_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x @ weight.T + bias`` with both operands in 8 bits and fp32 sums, rounded once.  ``x``: (..., K) fp32 / bf16 / fp16,
+    quantised inside as ``quantize_fp8`` does (the results are equal bit for bit), or ``Fp8Rows`` for rows that several products
+    share.  ``weight``: from ``quantize_fp8_weight``.  ``bias``: fp32 (N,).  ``out_dtype``: that of ``x`` by default (bf16 for
+    ``Fp8Rows``).  An operator of inference: it has no gradient, and refuses an ``x`` or ``bias`` that asks for one."""
+    rows, scale = (x.q, x.scale) if isinstance(x, Fp8Rows) else (x, None)
+    _on_gpu(rows, scale, weight.q, weight.scale, bias)
+    if torch.is_grad_enabled() and (rows.requires_grad or (bias is not None and bias.requires_grad)):
+        raise EvoDiffHipError("linear_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    return torch_ops.load().linear_fp8(rows, scale, weight.q, weight.scale, bias, out_dtype)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, select, top_k, n_classes):
+        logprob, entropy, top_logprob, top_token, stats = torch_ops.load().token_logprobs(logits, targets, select, top_k,
+                                                                                          n_classes, True)
+        ctx.save_for_backward(logits, targets, select, stats, entropy, top_token)
+        ctx.top_k, ctx.n_classes = top_k, n_classes
+        ctx.mark_non_differentiable(top_token)
+        ctx.set_materialize_grads(False)
+        return logprob, entropy, top_logprob, top_token
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprob, g_entropy, g_top, _):
+        logits, targets, select, stats, entropy, top_token = ctx.saved_tensors
+        grad = torch_ops.load().token_logprobs_backward(logits, targets, select, ctx.top_k, ctx.n_classes, stats, entropy,
+                                                        top_token, g_logprob if targets is not None else None, g_entropy,
+                                                        g_top)
+        return grad, None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top_k: int = 0,
+                   select: Optional[torch.Tensor] = None, n_classes: Optional[int] = None) -> TokenLogprobs:
+    """The log probability of ``targets`` under ``logits`` (..., V) fp32 / bf16 / fp16, with the entropy and the ``top_k``
+    alternatives (at most 32, equal values by lowest index) of every row, in one pass over the logits and fp32 sums.
+
+    ``targets``: int64, shaped like the logits without classes, or None.  ``select``: bool or uint8 of that shape; rows where it is
+    false are not read: results 0, tokens -1, gradient 0.  ``n_classes``: only the first ``n_classes`` classes count.
+    -inf forbids a class; a row without any other has logprob -inf, entropy 0, alternatives at -inf and no gradient.  A row with
+    NaN or +inf yields NaN, and so does a target outside [0, n_classes) for its logprob.  Logits may be a view with up to two
+    strided leading dimensions (``logits[:, :-1]``); others are copied first.
+
+    Differentiable once in ``logprob``, ``entropy`` and ``top_logprob``."""
+    _on_gpu(logits, targets, select)
+    if logits.dim() < 1:
+        raise ValueError("logits must have a dimension of classes")
+    n_classes = logits.shape[-1] if n_classes is None else int(n_classes)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = _TokenLogprobs.apply(logits, targets, select, int(top_k), n_classes)
+    else:
+        out = torch_ops.load().token_logprobs(logits.detach(), targets, select, int(top_k), n_classes, False)[:4]
+    return TokenLogprobs(out[0] if targets is not None else None, *out[1:])

@@ -1,5 +1,5 @@
 """The thin PyTorch-ROCm C++ extension over the C ABI: ``torch.ops.evodiff_amd.{forward, oadm_sample_, d3pm_sample_,
-score_nll}`` (evodiff_amd/csrc/torch_ops.cpp).  The operators take torch tensors, run on PyTorch's current HIP stream
+score_nll}`` and the model-free operators that ``evodiff_amd.ops`` wraps (evodiff_amd/csrc/torch_ops.cpp).  The operators take torch tensors, run on PyTorch's current HIP stream
 and raise ``RuntimeError`` on failure; ``handle`` is ``int(model.hip_handle(device).value)``.  The ctypes binding
 (``evodiff_amd._lib``) is the torch-free way to the same entry points; both go through ``libevodiff_hip.so``."""
 import os

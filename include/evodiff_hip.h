@@ -261,6 +261,74 @@ int ed_debug_set_stamp_buffer(int64_t* stamps_dev, int64_t n);
 int ed_debug_ln_act(const void* in_dev, int in_bf16, void* out_dev, int out_bf16, const float* gamma_dev,
                     const float* beta_dev, int rows, int C, int act, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Model-free operators (no counterpart in the reference): what a scoring or generation program runs on hidden states and
+ * logits of its own.  They need no model handle, keep no state and allocate nothing; the device that holds the buffers must
+ * be current (hipSetDevice).  Calls may overlap on any streams as long as they do not share a workspace.  Row strides are
+ * in elements and may exceed the row length; the last dimension is contiguous.  Float buffers are aligned to their element
+ * (quantised operands to 16 bytes).  Zero rows are a valid call that does nothing. */
+enum { ED_DT_FP32 = 0, ED_DT_BF16 = 1, ED_DT_FP16 = 2, ED_DT_E4M3 = 3 };
+
+/* Block-scaled 8-bit form.  Values are OCP e4m3 bytes (no infinities, largest 448), rounded to nearest even; 128 of them
+ * share a scale 2^(byte - 127), held as one E8M0 byte: the smallest power of two with which the block's largest finite
+ * magnitude stays within 448 (byte 1 .. 254; 1 for an all-zero block).  Infinities and NaN become NaN.  Rows are padded
+ * with zeros to Kb = ceil(K / 128) blocks.
+ *   rows (activations):  q_dev (rows, Kb * 128), scale_dev (rows, Kb): a scale for 128 channels of a row
+ *   weights:             q_dev (N, Kb * 128), scale_dev (ceil(N / 128), Kb): a scale for 128 x 128 */
+int ed_fp8_quantize_rows(const void* x_dev, int x_dtype, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q_dev,
+                         uint8_t* scale_dev, void* stream);
+int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, int64_t N, int64_t K, uint8_t* q_dev,
+                           uint8_t* scale_dev, void* stream);
+
+/* out (M, N) = x (M, K) @ weight (N, K)^T + bias, sums in fp32, rounded once to out_dtype (FP32, BF16 or FP16; contiguous).
+ * x_dtype ED_DT_E4M3: x_dev and x_scale_dev are rows in the form above (row_stride = Kb * 128).  Any other x_dtype: x_dev holds
+ * plain values, which are brought to that form first (x_scale_dev is ignored) - the result is the same, bit for bit, as
+ * of ed_fp8_quantize_rows and a product on its outputs.  bias_dev: fp32 [N] or NULL.
+ * workspace_dev: at least ed_fp8_linear_workspace(M, N, K, x_dtype) bytes, 16-byte aligned (NULL where that is 0); its contents
+ * do not matter before or after the call. */
+int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype);
+int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
+                  const uint8_t* weight_scale_dev, const float* bias_dev, void* out_dev, int out_dtype, int64_t M, int64_t N,
+                  int64_t K, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* Per row of logits (the first n_classes values of each): the log probability of targets[r], the entropy of the row's
+ * distribution (nats) and the top_k most likely classes, likeliest first, equal values by lowest index.
+ * Row r starts at logits + (r / inner_rows) * outer_stride + (r % inner_rows) * row_stride elements; inner_rows = rows for
+ * evenly spaced rows.  fp32 sums whatever the type.
+ *   -inf forbids a class (log probability -inf).  A row without any other class: logprob -inf, entropy 0, top
+ *   alternatives 0, 1, ... at -inf, gradient 0.  A row with NaN or +inf: logprob, entropy and top_logprob NaN, tokens
+ *   some class, gradient NaN.  A target outside [0, n_classes): logprob and gradient NaN, nothing is read there.
+ *   select_dev (rows bytes, may be NULL = every row): a row with a zero byte is not read; its results are 0, its tokens -1,
+ *   its gradient 0.
+ * targets_dev may be NULL: logprob_dev is then not written (and may be NULL).  logprob_dev, entropy_dev fp32 [rows];
+ * top_logprob_dev fp32, top_token_dev int64 [rows][top_k], top_k in [0, min(n_classes, ED_TOP_K_MAX)]; row_stats_dev
+ * fp32 [rows][2], or NULL where no gradient follows: the row's maximum and log sum exp(x - maximum).
+ * workspace_dev: at least ed_token_logprobs_workspace(rows, n_classes, top_k) bytes, 16-byte aligned (NULL where that is 0). */
+#define ED_TOP_K_MAX 32
+int64_t ed_token_logprobs_workspace(int64_t rows, int64_t n_classes, int top_k);
+int ed_token_logprobs(const void* logits_dev, int dtype, int64_t row_stride, int64_t inner_rows, int64_t outer_stride,
+                      int64_t rows, int64_t n_classes, const int64_t* targets_dev, const uint8_t* select_dev, int top_k,
+                      float* logprob_dev, float* entropy_dev, float* row_stats_dev, float* top_logprob_dev,
+                      int64_t* top_token_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
+/* The gradient of all of that to the logits: dlogits_dev (rows, columns) contiguous, of the logits' type, zeros in columns
+ * [n_classes, columns).  row_stats_dev, entropy_dev and top_token_dev as ed_token_logprobs wrote them for the same
+ * logits, targets, select and top_k.  grad_logprob_dev, grad_entropy_dev [rows], grad_top_dev [rows][top_k]: fp32, each may
+ * be NULL = zero.  No atomics: the result does not depend on any order. */
+int ed_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row_stride, int64_t inner_rows,
+                               int64_t outer_stride, int64_t rows, int64_t n_classes, int64_t columns,
+                               const int64_t* targets_dev, const uint8_t* select_dev, int top_k,
+                               const float* row_stats_dev, const float* entropy_dev, const int64_t* top_token_dev,
+                               const float* grad_logprob_dev, const float* grad_entropy_dev, const float* grad_top_dev,
+                               void* dlogits_dev, void* stream);
+
+/* ed_forward followed by ed_token_logprobs on its logits: for every position, the log probability of targets[b][l] over the
+ * first n_classes classes, the entropy there and the top_k alternatives; the sibling of ed_score_nll, which returns the
+ * negative log probability alone.  Same conventions as ed_score_nll for tokens, timesteps, targets and select (positions
+ * that are not selected: 0, tokens -1); the logits stay in the model's workspace. */
+int ed_score_tokens(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_dev, const int64_t* targets_dev,
+                    const uint8_t* select_dev, int B, int L, int n_classes, int top_k, float* logprob_dev,
+                    float* entropy_dev, float* top_logprob_dev, int64_t* top_token_dev, int precision, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
