@@ -13,6 +13,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr int TOP_MAX = 32;  // = ED_TOP_K_MAX
 
 template <int DT>
 struct Elem;
@@ -102,6 +103,10 @@ struct RowResult {
   __device__ __forceinline__ float logprob(float x) const { return bad ? __builtin_nanf("") : (x - m) - log_s; }
 };
 
+__device__ __forceinline__ void put_stats(float* to, float m, float log_s) {
+  to[0] = m;
+  to[1] = log_s;
+}
 __device__ __forceinline__ void skip_row(const LogprobsOut& out, long r, int top_k, int tid, int threads) {
   if (tid == 0) {
     if (out.logprob) out.logprob[r] = 0.f;
@@ -114,49 +119,236 @@ __device__ __forceinline__ void skip_row(const LogprobsOut& out, long r, int top
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void logprobs_row_kernel(LogitsView x, const int64_t* __restrict__ targets,
-                                                           const uint8_t* __restrict__ select, int top_k,
-                                                           LogprobsOut out) {
+// ---------------------------------------------------------------------------------------------------
+// Few classes (n <= G * E <= 1024): G lanes own a row and keep it in registers, lane j the classes j, j + G, ...
+// ---------------------------------------------------------------------------------------------------
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+
+template <int DT, int G, int E>
+__global__ __launch_bounds__(256) void logprobs_group_kernel(LogitsView x, const int64_t* __restrict__ targets,
+                                                             const uint8_t* __restrict__ select, int top_k,
+                                                             LogprobsOut out) {
   typedef typename Elem<DT>::T T;
-  __shared__ Sums sums[256];
-  __shared__ unsigned long long keys[256];
-  const int tid = threadIdx.x;
-  for (long r = blockIdx.x; r < x.rows; r += gridDim.x) {
-  __syncthreads();
-  if (select && !select[r]) {
-    skip_row(out, r, top_k, tid, 256);
-    continue;
-  }
-  const T* row = row_of<T>(x, r);
-  Sums a;
-  a.clear();
-  for (int v = tid; v < x.n; v += 256) a.add(Elem<DT>::get(row[v]));
-  sums[tid] = a;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) sums[tid].join(sums[tid + o]);
-    __syncthreads();
-  }
-  const RowResult res(sums[0]);
-  if (tid == 0) {
-    if (targets) {
-      const int64_t t = targets[r];
-      out.logprob[r] = t < 0 || t >= x.n ? __builtin_nanf("") : res.logprob(Elem<DT>::get(row[t]));
+  const int lane = threadIdx.x & (G - 1);
+  for (long r = (long)blockIdx.x * (256 / G) + threadIdx.x / G; r < x.rows; r += (long)gridDim.x * (256 / G)) {
+    if (select && !select[r]) {
+      skip_row(out, r, top_k, lane, G);
+      continue;
     }
-    out.entropy[r] = res.entropy;
-    if (out.stats) {
-      out.stats[2 * r] = res.mark();
-      out.stats[2 * r + 1] = res.log_s;
+    const T* row = row_of<T>(x, r);
+    const int64_t target = targets ? targets[r] : -1;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e * G + lane < x.n ? Elem<DT>::get(row[e * G + lane]) : NEG_INF;
+    const float xt = target >= 0 && target < x.n ? Elem<DT>::get(row[target]) : __builtin_nanf("");
+    Sums a;
+    a.m = v[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) a.m = fmaxf(a.m, v[e]);
+    a.m = group_max<G>(a.m);
+    a.s = a.t = 0.f;
+    const float m = a.m == NEG_INF ? 0.f : a.m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = v[e] - m, p = exp2f(d * LOG2E);
+      a.s += p;
+      a.t = fmaf(fmaxf(d, -1.0e30f), p, a.t);
+    }
+    a.s = group_sum<G>(a.s);
+    a.t = group_sum<G>(a.t);
+    const RowResult res(a);
+    if (lane == 0) {
+      if (targets) out.logprob[r] = res.logprob(xt);
+      out.entropy[r] = res.entropy;
+      if (out.stats) put_stats(out.stats + 2 * r, res.mark(), res.log_s);
+    }
+    if (top_k == 0) continue;
+    unsigned key[E];  // order of the values; 0: taken, or no class
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = e * G + lane < x.n ? (unsigned)(key_of(v[e], 0) >> 32) : 0u;
+    for (int j = 0; j < top_k; ++j) {
+      unsigned best = key[0];
+      int at = 0;
+#pragma unroll
+      for (int e = 1; e < E; ++e)
+        if (key[e] > best) {
+          best = key[e];
+          at = e;
+        }
+      int idx = at * G + lane;
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) {
+        const unsigned b = (unsigned)__shfl_xor((int)best, o);
+        const int i = __shfl_xor(idx, o);
+        const bool take = b > best || (b == best && i < idx);
+        best = take ? b : best;
+        idx = take ? i : idx;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * G + lane == idx) key[e] = 0u;
+      if (lane == 0) {
+        out.top_logprob[r * top_k + j] = res.logprob(key_value((unsigned long long)best << 32));
+        out.top_token[r * top_k + j] = idx;
+      }
     }
   }
-  unsigned long long last = ~0ull;
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Many classes: one pass of 16-byte loads by a workgroup per row, or per piece of a row where there are few rows (the
+// pieces are joined by a second kernel).
+//
+// Sums.  In base 2: y = x * log2(e) - R with one fused operation, R = M * log2(e) for M the wave's largest value so far, S = sum
+// 2^y, T = sum y 2^y.  (log2(e) is off by 1.3e-8 relative in fp32, as if every logit were scaled by that: under one rounding of
+// a log probability.)  y is kept at -200 or above, so that a forbidden class adds nothing and not a NaN.  Values of 2^20 and
+// more leave the products too coarse: a row with such a maximum is summed once more, plainly.
+//
+// Top alternatives.  A group is the contiguous classes of one load; the k largest values lie in the k groups with the largest
+// maxima, and as groups are ordered as their classes are, ties go the same way.  Every thread keeps its best group; the k-th
+// of them (joined over the four waves: 64) is a bound tau that at least k groups reach, renewed after 1, 2, 4, ... tiles.
+// Groups that reach it go to a list, about 1.2 k for each doubling; in the end those that reach the last tau are read
+// again, class by class, and ranked by counting.  A list that overflows (rows in rising order) takes k plain passes.
+// ---------------------------------------------------------------------------------------------------
+constexpr float Y_MIN = -200.0f, R_MIN = -2097152.0f, PLAIN_FROM = 1048576.0f;
+constexpr int LIST = 512, GROUPS = 64;
+typedef unsigned long long u64;
+
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // a NaN stays one
+
+// Sums of a wave, workgroup or row in base 2.
+struct Sums2 {
+  float m, r, s, t;  // largest value, reference, sum 2^y, sum y 2^y
+  __device__ __forceinline__ void rebase(float to) {
+    const float d = r - to, f = __builtin_amdgcn_exp2f(d);
+    t = f * fmaf(d, s, t);
+    s *= f;
+    r = to;
+  }
+  __device__ __forceinline__ void join(Sums2 o) {
+    const float to = fmaxf(r, o.r);
+    rebase(to);
+    o.rebase(to);
+    s += o.s;
+    t += o.t;
+    m = fmaxf(m, o.m);
+  }
+};
+
+struct RowEnd {  // what follows from the sums of a whole row
+  float m, log_s, entropy;
+  bool empty, bad;
+  __device__ __forceinline__ RowEnd(const Sums2& a) {
+    empty = a.m == NEG_INF && a.s == 0.f;
+    bad = !empty && !(a.s > 0.f && a.s < __builtin_huge_valf());
+    const float l2 = __builtin_amdgcn_logf(a.s);
+    m = empty ? 0.f : a.m;
+    log_s = empty ? 0.f : bad ? __builtin_nanf("") : (l2 - fmaf(a.m, LOG2E, -a.r)) * LN2;
+    entropy = empty ? 0.f : bad ? __builtin_nanf("") : (l2 - a.t / a.s) * LN2;
+  }
+  __device__ __forceinline__ RowEnd(const RowResult& a) : m(a.m), log_s(a.log_s), entropy(a.entropy), empty(a.empty), bad(a.bad) {}
+  __device__ __forceinline__ float mark() const { return empty ? NEG_INF : bad ? __builtin_nanf("") : m; }
+  __device__ __forceinline__ float logprob(float x) const { return bad ? __builtin_nanf("") : (x - m) - log_s; }
+};
+
+// The 16-byte loads of a row: classes [0, head) and [n - tail, n) stand alone, the rest are vectors of EPV.
+template <int DT>
+struct Vectors {
+  typedef typename Elem<DT>::T T;
+  static constexpr int EPV = 16 / sizeof(T);
+  const T* row;
+  int n, head, count;  // vectors
+  __device__ __forceinline__ Vectors(const T* p, int classes) : row(p), n(classes) {
+    head = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+    head = head < n ? head : n;
+    count = (n - head) / EPV;
+  }
+  __device__ __forceinline__ int tail() const { return n - head - count * EPV; }
+  __device__ __forceinline__ int first(int v) const { return head + v * EPV; }  // class of vector v
+  __device__ __forceinline__ bool single(int e) const { return e < head || e >= head + count * EPV; }
+};
+
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[16 / sizeof(typename Elem<DT>::T)]) {
+  if constexpr (DT == DT_FP32) {
+    v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y); v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
+  } else {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == DT_BF16) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)w[i]);
+        v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[i] >> 16));
+      }
+    }
+  }
+}
+
+struct TopSpace {
+  u64 best[256];               // a thread's best group
+  u64 list[LIST];              // groups that reached tau
+  u64 found[GROUPS * 8];       // classes that may be among the k
+  int group[GROUPS];
+  u64 tau;
+  int listed, groups, n_found;
+};
+
+// tau = the k-th of the 64 best groups (0, which every group reaches, where there are fewer)
+__device__ __forceinline__ void renew_tau(TopSpace& sp, u64 mine, int top_k, int tid) {
+  sp.best[tid] = mine;
+  __syncthreads();
+  if (tid < 64) {
+    const u64 k = max_key(max_key(sp.best[tid], sp.best[tid + 64]), max_key(sp.best[tid + 128], sp.best[tid + 192]));
+    sp.best[tid] = k;
+    __builtin_amdgcn_wave_barrier();
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) rank += sp.best[j] > k;
+    if (rank == top_k - 1 && k) sp.tau = k;
+  }
+  __syncthreads();
+}
+
+// out[rank] = the k largest of sp.found[0 .. n) in order, by counting; n >= k
+template <typename Put>
+__device__ __forceinline__ void rank_found(const u64* found, int n, int top_k, int tid, Put put) {
+  for (int i = tid; i < n; i += 256) {
+    const u64 k = found[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += found[j] > k;
+    if (rank < top_k) put(rank, k);
+  }
+}
+
+// k plain passes over classes [from, to) (and [from2, to2)), each for the largest below the one before
+template <int DT, typename Put>
+__device__ void plain_top(const typename Elem<DT>::T* row, int from, int to, int from2, int to2, int top_k, u64* keys, int tid, Put put) {
+  u64 last = ~0ull;
   for (int j = 0; j < top_k; ++j) {
-    unsigned long long best = 0;
-    for (int v = tid; v < x.n; v += 256) {
-      const unsigned long long k = key_of(Elem<DT>::get(row[v]), v);
+    u64 best = 0;
+    for (int v = from + tid; v < to; v += 256) {
+      const u64 k = key_of(Elem<DT>::get(row[v]), v);
       if (k < last) best = max_key(best, k);
     }
+    for (int v = from2 + tid; v < to2; v += 256) {
+      const u64 k = key_of(Elem<DT>::get(row[v]), v);
+      if (k < last) best = max_key(best, k);
+    }
+    __syncthreads();
     keys[tid] = best;
     __syncthreads();
     for (int o = 128; o > 0; o >>= 1) {
@@ -164,12 +356,297 @@ __global__ __launch_bounds__(256) void logprobs_row_kernel(LogitsView x, const i
       __syncthreads();
     }
     last = keys[0];
+    if (tid == 0) put(j, last);
+  }
+  __syncthreads();
+}
+
+// a row's sums without base 2 and vectors, for maxima of any size
+template <int DT>
+__device__ RowResult plain_sums(const typename Elem<DT>::T* row, int n, float* space, int tid) {
+  Sums a;
+  a.clear();
+  for (int v = tid; v < n; v += 256) a.add(Elem<DT>::get(row[v]));
+  __syncthreads();
+  space[tid] = a.m; space[256 + tid] = a.s; space[512 + tid] = a.t;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) {
+      Sums b;
+      a.m = space[tid]; a.s = space[256 + tid]; a.t = space[512 + tid];
+      b.m = space[tid + o]; b.s = space[256 + tid + o]; b.t = space[512 + tid + o];
+      a.join(b);
+      space[tid] = a.m; space[256 + tid] = a.s; space[512 + tid] = a.t;
+    }
     __syncthreads();
-    if (tid == 0) {
-      out.top_logprob[r * top_k + j] = res.logprob(key_value(last));
-      out.top_token[r * top_k + j] = key_index(last);
+  }
+  a.m = space[0]; a.s = space[256]; a.t = space[512];
+  __syncthreads();
+  return RowResult(a);
+}
+
+struct Piece {  // of a row: its sums, followed in memory by top_k keys
+  Sums2 sums;
+};
+__host__ __device__ inline long piece_bytes(int top_k) { return (long)sizeof(Piece) + 8L * top_k; }
+
+template <int DT, bool TOP>
+__global__ __launch_bounds__(256) void logprobs_stream_kernel(LogitsView x, const int64_t* __restrict__ targets,
+                                                              const uint8_t* __restrict__ select, int top_k,
+                                                              LogprobsOut out, char* __restrict__ pieces, int splits) {
+  typedef typename Elem<DT>::T T;
+  constexpr int EPV = Vectors<DT>::EPV, U = 4;
+  __shared__ TopSpace sp;
+  __shared__ Sums2 wave_sums[4];
+  __shared__ float plain_space[768];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const long items = x.rows * splits;
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long r = item / splits;
+    const int piece = (int)(item - r * splits);
+    if (select && !select[r]) {
+      if (piece == 0 && splits == 1) skip_row(out, r, top_k, tid, 256);
+      continue;
+    }
+    const Vectors<DT> vec(row_of<T>(x, r), x.n);
+    const int chunk = (vec.count + splits - 1) / splits;
+    const int v0 = piece * chunk < vec.count ? piece * chunk : vec.count;
+    const int v1 = v0 + chunk < vec.count ? v0 + chunk : vec.count;
+    const uint4* src = (const uint4*)(vec.row + vec.head);
+    const unsigned none = DT == DT_FP32 ? 0xff800000u : DT == DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+
+    __syncthreads();  // the row before is done with the shared memory
+    if (TOP && tid == 0) {
+      sp.tau = 0;
+      sp.listed = sp.groups = sp.n_found = 0;
+    }
+    Sums2 a{NEG_INF, R_MIN, 0.f, 0.f};
+    auto raise = [&](float v) {  // a larger value somewhere in the wave: new reference
+      a.m = fmaxf(a.m, v);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) a.m = fmaxf(a.m, __shfl_xor(a.m, o));
+      a.rebase(fmaxf(a.m * LOG2E, R_MIN));
+    };
+    auto add = [&](float v) {
+      const float y = max_nan(fmaf(v, LOG2E, -a.r), Y_MIN), e = __builtin_amdgcn_exp2f(y);
+      a.s += e;
+      a.t = fmaf(y, e, a.t);
+    };
+    // classes in front of and behind the vectors
+    float alone = NEG_INF;
+    int alone_at = -1;
+    if (piece == 0) {
+      if (tid < vec.head) alone_at = tid;
+      else if (tid >= 64 && tid - 64 < vec.tail()) alone_at = vec.n - vec.tail() + tid - 64;
+      if (alone_at >= 0) alone = Elem<DT>::get(vec.row[alone_at]);
+      if (__any(alone > a.m)) raise(alone);
+      add(alone);
+      if (TOP) {
+        __syncthreads();
+        if (alone_at >= 0) sp.list[atomicAdd(&sp.listed, 1)] = key_of(alone, alone_at);
+      }
+    }
+
+    uint4 raw[U], next[U];
+    auto load = [&](uint4 (&to)[U], int at) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = at + u * 256 + tid;
+        to[u] = v < v1 ? src[v] : make_uint4(none, none, none, none);
+      }
+    };
+    float best = NEG_INF, tau_value = NEG_INF;  // this thread's best group
+    int best_at = -1, tiles = 0, renew_at = 1;
+    u64 tau = 0;
+    load(next, v0);
+    for (int at = v0; at < v1; at += 256 * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      load(next, at + 256 * U);
+      float high[U];
+      float v[EPV];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        unpack<DT>(raw[u], v);
+        high[u] = v[0];
+#pragma unroll
+        for (int i = 1; i < EPV; ++i) high[u] = fmaxf(high[u], v[i]);
+      }
+      const float top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+      if (__any(top > a.m)) raise(top);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        unpack<DT>(raw[u], v);
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) add(v[i]);
+      }
+      if constexpr (TOP) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int g = at + u * 256 + tid;
+          if (g < v1 && (high[u] > best || best_at < 0)) {
+            best = high[u];
+            best_at = vec.first(g);
+          }
+        }
+        if (++tiles == renew_at || at + 256 * U >= v1) {
+          renew_tau(sp, best_at < 0 ? 0 : key_of(best, best_at), top_k, tid);
+          tau = sp.tau;
+          tau_value = tau ? key_value(tau) : NEG_INF;
+          renew_at *= 2;
+        }
+        if (__any(top >= tau_value)) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int g = at + u * 256 + tid;
+            const u64 k = key_of(high[u], vec.first(g));
+            const bool take = g < v1 && k >= tau;
+            const u64 mask = __ballot(take);
+            if (mask) {
+              int base = 0;
+              if (lane == (int)__builtin_ctzll(mask)) base = atomicAdd(&sp.listed, (int)__popcll(mask));
+              base = __shfl(base, (int)__builtin_ctzll(mask));
+              const int pos = base + (int)__popcll(mask & ((1ull << lane) - 1));
+              if (take && pos < LIST) sp.list[pos] = k;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      a.s += __shfl_xor(a.s, o);
+      a.t += __shfl_xor(a.t, o);
+    }
+    if (lane == 0) wave_sums[wid] = a;
+    __syncthreads();
+    a = wave_sums[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) a.join(wave_sums[w]);
+
+    char* const mine = pieces + item * piece_bytes(top_k);
+    if (splits > 1) {
+      if (tid == 0) ((Piece*)mine)->sums = a;
+    }
+    const bool plain = splits == 1 && (a.m > PLAIN_FROM || a.m < -PLAIN_FROM) && a.m != NEG_INF;
+    const RowEnd res = plain ? RowEnd(plain_sums<DT>(vec.row, vec.n, plain_space, tid)) : RowEnd(a);
+    if (splits == 1 && tid == 0) {
+      if (targets) {
+        const int64_t t = targets[r];
+        out.logprob[r] = t < 0 || t >= x.n ? __builtin_nanf("") : res.logprob(Elem<DT>::get(vec.row[t]));
+      }
+      out.entropy[r] = res.entropy;
+      if (out.stats) put_stats(out.stats + 2 * r, res.mark(), res.log_s);
+    }
+    if constexpr (TOP) {
+      auto put = [&](int rank, u64 k) {
+        if (splits > 1) {
+          ((u64*)(mine + sizeof(Piece)))[rank] = k;
+        } else {
+          out.top_logprob[r * top_k + rank] = res.logprob(key_value(k));
+          out.top_token[r * top_k + rank] = key_index(k);
+        }
+      };
+      const int listed = sp.listed;
+      bool fits = listed <= LIST;
+      if (fits) {
+        for (int i = tid; i < listed; i += 256) {
+          const u64 k = sp.list[i];
+          if (k >= tau) {
+            const int pos = atomicAdd(&sp.groups, 1);
+            if (pos < GROUPS) sp.group[pos] = key_index(k);
+          }
+        }
+        __syncthreads();
+        const int groups = sp.groups;
+        fits = groups <= GROUPS;
+        if (fits) {
+          // at least k classes reach (value of tau, last class of its group)
+          const u64 floor = tau ? tau - (EPV - 1) : 0;
+          for (int i = tid; i < groups * EPV; i += 256) {
+            const int e0 = sp.group[i / EPV], e = e0 + i % EPV;
+            if (vec.single(e0) && e != e0) continue;
+            const u64 k = key_of(Elem<DT>::get(vec.row[e]), e);
+            if (k >= floor) sp.found[atomicAdd(&sp.n_found, 1)] = k;
+          }
+          __syncthreads();
+          const int n = sp.n_found;
+          rank_found(sp.found, n, top_k, tid, put);
+          // a piece may hold fewer classes than k (or a NaN may have hidden some)
+          for (int j = n + tid; j < top_k; j += 256) put(j, splits > 1 ? 0 : key_of(NEG_INF, 0));
+        }
+      }
+      if (!fits) {
+        const bool ends = piece == 0;
+        plain_top<DT>(vec.row, ends ? 0 : vec.first(v0), vec.first(v1), ends ? vec.n - vec.tail() : vec.n, vec.n, top_k, sp.best, tid,
+                      [&](int j, u64 k) { put(j, k || splits > 1 ? k : key_of(NEG_INF, 0)); });
+      }
     }
   }
+}
+
+// The pieces of a row: sums joined in order; of the sorted lists, the k-th of their first ceil(k / splits) entries each is a
+// bound that k classes reach.
+template <int DT>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const int64_t* __restrict__ targets,
+                                                            const uint8_t* __restrict__ select, int top_k, LogprobsOut out,
+                                                            const char* __restrict__ pieces, int splits) {
+  typedef typename Elem<DT>::T T;
+  __shared__ u64 keys[64 * TOP_MAX];
+  __shared__ u64 found[64 * TOP_MAX];
+  __shared__ u64 tau;
+  __shared__ int n_found;
+  __shared__ float plain_space[768];
+  const int tid = threadIdx.x;
+  for (long r = blockIdx.x; r < x.rows; r += gridDim.x) {
+    if (select && !select[r]) {
+      skip_row(out, r, top_k, tid, 256);
+      continue;
+    }
+    const T* row = row_of<T>(x, r);
+    const char* src = pieces + r * splits * piece_bytes(top_k);
+    __syncthreads();
+    if (tid == 0) {
+      tau = 0;
+      n_found = 0;
+    }
+    for (int i = tid; i < splits * top_k; i += 256) {
+      const int s = i / top_k;
+      keys[i] = ((const u64*)(src + s * piece_bytes(top_k) + sizeof(Piece)))[i - s * top_k];
+    }
+    Sums2 a = ((const Piece*)src)->sums;
+    for (int s = 1; s < splits; ++s) a.join(((const Piece*)(src + s * piece_bytes(top_k)))->sums);
+    const bool plain = (a.m > PLAIN_FROM || a.m < -PLAIN_FROM) && a.m != NEG_INF;
+    const RowEnd res = plain ? RowEnd(plain_sums<DT>(row, x.n, plain_space, tid)) : RowEnd(a);
+    if (tid == 0) {
+      if (targets) {
+        const int64_t t = targets[r];
+        out.logprob[r] = t < 0 || t >= x.n ? __builtin_nanf("") : res.logprob(Elem<DT>::get(row[t]));
+      }
+      out.entropy[r] = res.entropy;
+      if (out.stats) put_stats(out.stats + 2 * r, res.mark(), res.log_s);
+    }
+    if (top_k == 0) continue;
+    __syncthreads();
+    const int depth = (top_k + splits - 1) / splits, firsts = depth * splits;  // firsts < splits + top_k <= 96
+    if (tid < firsts) {
+      const u64 k = keys[(tid / depth) * top_k + tid % depth];
+      int rank = 0;
+      for (int j = 0; j < firsts; ++j) rank += keys[(j / depth) * top_k + j % depth] > k;
+      if (rank == top_k - 1 && k) tau = k;
+    }
+    __syncthreads();
+    const u64 floor = tau;
+    for (int i = tid; i < splits * top_k; i += 256)
+      if (keys[i] && keys[i] >= floor) found[atomicAdd(&n_found, 1)] = keys[i];
+    __syncthreads();
+    auto put = [&](int rank, u64 k) {
+      out.top_logprob[r * top_k + rank] = res.logprob(key_value(k));
+      out.top_token[r * top_k + rank] = key_index(k);
+    };
+    const int n = n_found;
+    rank_found(found, n, top_k, tid, put);
+    for (int j = n + tid; j < top_k; j += 256) put(j, key_of(NEG_INF, 0));
   }
 }
 
@@ -208,15 +685,55 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
 
 }  // namespace
 
-int64_t token_logprobs_workspace(int64_t rows, int64_t n, int top_k) { return 0; }
+// Pieces of a row: one where the rows alone give every CU two workgroups; else as many as bring the grid there, none under 4096
+// classes (under two 16-byte loads a thread a piece costs more than it saves), at most 64.
+static int row_splits(int64_t rows, int64_t n) {
+  if (n <= 1024) return 1;
+  const int64_t want = (512 + rows - 1) / rows, most = (n + 4095) / 4096;
+  const int64_t s = want < most ? want : most;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+int64_t token_logprobs_workspace(int64_t rows, int64_t n, int top_k) {
+  const int splits = row_splits(rows, n);
+  return splits > 1 ? rows * splits * piece_bytes(top_k) : 0;
+}
+
+template <int DT>
+static hipError_t launch_logprobs(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
+                                  const LogprobsOut& out, void* workspace, hipStream_t stream) {
+  auto blocks = [&](long n) { return dim3((unsigned)(n < (1 << 20) ? n : 1 << 20)); };
+#define ED_GROUP(G, E)                                                                                                     \
+  hipLaunchKernelGGL((logprobs_group_kernel<DT, G, E>), blocks((x.rows + 256 / G - 1) / (256 / G)), dim3(256), 0, stream, x, \
+                     targets, select, top_k, out)
+  if (x.n <= 32) ED_GROUP(4, 8);
+  else if (x.n <= 64) ED_GROUP(8, 8);
+  else if (x.n <= 256) ED_GROUP(16, 16);
+  else if (x.n <= 1024) ED_GROUP(64, 16);
+  else {
+    const int splits = row_splits(x.rows, x.n);
+    if (top_k > 0)
+      hipLaunchKernelGGL((logprobs_stream_kernel<DT, true>), blocks(x.rows * splits), dim3(256), 0, stream, x, targets, select, top_k,
+                         out, (char*)workspace, splits);
+    else
+      hipLaunchKernelGGL((logprobs_stream_kernel<DT, false>), blocks(x.rows * splits), dim3(256), 0, stream, x, targets, select, top_k,
+                         out, (char*)workspace, splits);
+    if (splits > 1) {
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL((logprobs_join_kernel<DT>), blocks(x.rows), dim3(256), 0, stream, x, targets, select, top_k, out,
+                         (const char*)workspace, splits);
+    }
+  }
+#undef ED_GROUP
+  return hipGetLastError();
+}
 
 hipError_t launch_token_logprobs(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
                                  const LogprobsOut& out, void* workspace, hipStream_t stream) {
-  const dim3 grid((unsigned)(x.rows < (1 << 20) ? x.rows : 1 << 20));
-  if (x.dt == DT_FP32) hipLaunchKernelGGL((logprobs_row_kernel<DT_FP32>), grid, dim3(256), 0, stream, x, targets, select, top_k, out);
-  else if (x.dt == DT_BF16) hipLaunchKernelGGL((logprobs_row_kernel<DT_BF16>), grid, dim3(256), 0, stream, x, targets, select, top_k, out);
-  else hipLaunchKernelGGL((logprobs_row_kernel<DT_FP16>), grid, dim3(256), 0, stream, x, targets, select, top_k, out);
-  return hipGetLastError();
+  if (x.dt == DT_FP32) return launch_logprobs<DT_FP32>(x, targets, select, top_k, out, workspace, stream);
+  if (x.dt == DT_BF16) return launch_logprobs<DT_BF16>(x, targets, select, top_k, out, workspace, stream);
+  return launch_logprobs<DT_FP16>(x, targets, select, top_k, out, workspace, stream);
 }
 
 hipError_t launch_token_logprobs_backward(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
