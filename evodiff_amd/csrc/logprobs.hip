@@ -650,36 +650,109 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
   }
 }
 
+// ---------------------------------------------------------------------------------------------------
+// Gradient: a value in, a value out.  log p comes from the row's saved maximum and log sum; the few classes that are named
+// (target, top alternatives) are written once more behind the rest of their tile by the workgroup that owns it, each as the
+// whole sum for its class, in a fixed order.
+// ---------------------------------------------------------------------------------------------------
+struct GradRow {
+  float m, log_s, h, weight, g_h;
+  bool skip;
+  __device__ __forceinline__ float at(float x) const {
+    const float lp = (x - m) - log_s, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    return -p * fmaf(g_h, max_nan(lp, -1.0e30f) + h, weight);  // (a forbidden class: nothing, not nothing times infinity)
+  }
+};
+__device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
+                                            const LogprobsGrad& g, long r) {
+  GradRow a;
+  a.m = g.stats[2 * r];
+  a.log_s = g.stats[2 * r + 1];
+  a.skip = (select && !select[r]) || a.m == NEG_INF;
+  a.h = g.entropy[r];
+  a.weight = g.g_logprob ? g.g_logprob[r] : 0.f;
+  a.g_h = g.g_entropy ? g.g_entropy[r] : 0.f;
+  if (g.g_top)
+    for (int j = 0; j < top_k; ++j) a.weight += g.g_top[r * top_k + j];
+  if (targets && (targets[r] < 0 || targets[r] >= x.n)) a.weight = __builtin_nanf("");
+  return a;
+}
+// what the named classes of row r add to class v
+__device__ __forceinline__ float named(const int64_t* targets, int top_k, const LogprobsGrad& g, long r, int64_t v) {
+  float d = g.g_logprob && targets[r] == v ? g.g_logprob[r] : 0.f;
+  if (g.g_top)
+    for (int j = 0; j < top_k; ++j)
+      if (g.top_token[r * top_k + j] == v) d += g.g_top[r * top_k + j];
+  return d;
+}
+
+// A workgroup per tile of 2048 / 4096 classes of a row: four 16-byte loads and stores a thread, where source and destination
+// rows lie alike within 16 bytes; class by class elsewhere.
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const int64_t* __restrict__ targets,
                                                             const uint8_t* __restrict__ select, int top_k,
-                                                            LogprobsGrad g) {
+                                                            LogprobsGrad g, int tiles) {
   typedef typename Elem<DT>::T T;
+  constexpr int EPV = 16 / sizeof(T), U = 2, TILE = 256 * U * EPV;
+  typedef __attribute__((ext_vector_type(EPV))) T VT;
   const int tid = threadIdx.x;
-  for (long r = blockIdx.x; r < x.rows; r += gridDim.x) {
-  const T* row = row_of<T>(x, r);
-  T* dst = (T*)g.dlogits + r * g.columns;
-  const bool skip = (select && !select[r]) || g.stats[2 * r] == NEG_INF;
-  const float m = g.stats[2 * r], log_s = g.stats[2 * r + 1], h = g.entropy[r];
-  const float g_lp = g.g_logprob ? g.g_logprob[r] : 0.f, g_h = g.g_entropy ? g.g_entropy[r] : 0.f;
-  const int64_t t = targets ? targets[r] : 0;
-  float weight = g_lp;
-  if (g.g_top)
-    for (int j = 0; j < top_k; ++j) weight += g.g_top[r * top_k + j];
-  if (t < 0 || t >= x.n) weight = __builtin_nanf("");
-  for (int v = tid; v < g.columns; v += 256) {
-    float d = 0.f;
-    if (!skip && v < x.n) {
-      const float lp = (Elem<DT>::get(row[v]) - m) - log_s;
-      const float p = exp2f(lp * LOG2E);
-      d = p == 0.f ? 0.f * weight : -p * (weight + g_h * (lp + h));
-      if (v == t) d += g_lp;
-      if (g.g_top)
-        for (int j = 0; j < top_k; ++j)
-          if (g.top_token[r * top_k + j] == v) d += g.g_top[r * top_k + j];
+  const long items = x.rows * tiles;
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long r = item / tiles;
+    const int tile = (int)(item - r * tiles);
+    const T* row = row_of<T>(x, r);
+    T* dst = (T*)g.dlogits + r * g.columns;
+    const GradRow a = grad_row(x, targets, select, top_k, g, r);
+    const int head = (int)((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / (int)sizeof(T);
+    const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
+    // this tile's columns: vectors are counted from the first aligned column, tile 0 also holds the ones in front
+    const long from = tile == 0 ? 0 : head + (long)tile * TILE, end = head + (long)(tile + 1) * TILE;
+    const long to = end < g.columns ? end : g.columns;
+    if (a.skip) {
+      for (long v = from + tid; v < to; v += 256) dst[v] = Elem<DT>::put(0.f);
+      continue;
     }
-    dst[v] = Elem<DT>::put(d);
+    if (alike && from + (tile == 0 ? head : 0) + TILE <= x.n) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long v = head + (long)tile * TILE + (u * 256 + tid) * EPV;
+        const uint4 raw = *(const uint4*)(row + v);
+        float f[EPV];
+        unpack<DT>(raw, f);
+        VT o;
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) o[i] = Elem<DT>::put(a.at(f[i]));
+        *(VT*)(dst + v) = o;
+      }
+      if (tile == 0 && tid < head) dst[tid] = Elem<DT>::put(a.at(Elem<DT>::get(row[tid])));
+    } else {
+      for (long v = from + tid; v < to; v += 256) dst[v] = Elem<DT>::put(v < x.n ? a.at(Elem<DT>::get(row[v])) : 0.f);
+    }
+    const int names = (g.g_logprob ? 1 : 0) + (g.g_top ? top_k : 0);
+    if (names) {
+      __syncthreads();  // (also waits for the stores above)
+      if (tid < names) {
+        const int64_t v = g.g_logprob && tid == 0 ? targets[r] : g.top_token[r * top_k + tid - (g.g_logprob ? 1 : 0)];
+        if (v >= from && v < to && v < x.n) dst[v] = Elem<DT>::put(a.at(Elem<DT>::get(row[v])) + named(targets, top_k, g, r, v));
+      }
+    }
   }
+}
+
+// Few columns: a thread per value, rows behind each other.
+template <int DT>
+__global__ __launch_bounds__(256) void logprobs_grad_flat_kernel(LogitsView x, const int64_t* __restrict__ targets,
+                                                                 const uint8_t* __restrict__ select, int top_k,
+                                                                 LogprobsGrad g) {
+  typedef typename Elem<DT>::T T;
+  const long count = x.rows * g.columns;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
+    const long r = i / g.columns;
+    const int v = (int)(i - r * g.columns);
+    const GradRow a = grad_row(x, targets, select, top_k, g, r);
+    float d = 0.f;
+    if (!a.skip && v < x.n) d = a.at(Elem<DT>::get(row_of<T>(x, r)[v])) + named(targets, top_k, g, r, v);
+    ((T*)g.dlogits)[i] = Elem<DT>::put(d);
   }
 }
 
@@ -736,13 +809,26 @@ hipError_t launch_token_logprobs(const LogitsView& x, const int64_t* targets, co
   return launch_logprobs<DT_FP16>(x, targets, select, top_k, out, workspace, stream);
 }
 
+template <int DT>
+static hipError_t launch_grad(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k, const LogprobsGrad& g,
+                              hipStream_t stream) {
+  auto blocks = [&](long n) { return dim3((unsigned)(n < (1 << 20) ? n : 1 << 20)); };
+  if (g.columns <= 256) {
+    hipLaunchKernelGGL((logprobs_grad_flat_kernel<DT>), blocks((x.rows * g.columns + 255) / 256), dim3(256), 0, stream, x, targets,
+                       select, top_k, g);
+  } else {
+    const long tile = 256 * 2 * (16 / dt_bytes(DT));
+    const int tiles = (int)((g.columns + tile - 1) / tile);  // (the columns in front of the first aligned one are tile 0's)
+    hipLaunchKernelGGL((logprobs_grad_kernel<DT>), blocks(x.rows * tiles), dim3(256), 0, stream, x, targets, select, top_k, g, tiles);
+  }
+  return hipGetLastError();
+}
+
 hipError_t launch_token_logprobs_backward(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
                                           const LogprobsGrad& g, hipStream_t stream) {
-  const dim3 grid((unsigned)(x.rows < (1 << 20) ? x.rows : 1 << 20));
-  if (x.dt == DT_FP32) hipLaunchKernelGGL((logprobs_grad_kernel<DT_FP32>), grid, dim3(256), 0, stream, x, targets, select, top_k, g);
-  else if (x.dt == DT_BF16) hipLaunchKernelGGL((logprobs_grad_kernel<DT_BF16>), grid, dim3(256), 0, stream, x, targets, select, top_k, g);
-  else hipLaunchKernelGGL((logprobs_grad_kernel<DT_FP16>), grid, dim3(256), 0, stream, x, targets, select, top_k, g);
-  return hipGetLastError();
+  if (x.dt == DT_FP32) return launch_grad<DT_FP32>(x, targets, select, top_k, g, stream);
+  if (x.dt == DT_BF16) return launch_grad<DT_BF16>(x, targets, select, top_k, g, stream);
+  return launch_grad<DT_FP16>(x, targets, select, top_k, g, stream);
 }
 
 }  // namespace ed
