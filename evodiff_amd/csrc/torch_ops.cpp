@@ -9,6 +9,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -258,67 +260,106 @@ RowInputs row_inputs(const at::Tensor& logits, const c10::optional<at::Tensor>& 
   return r;
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
-    const at::Tensor& logits, const c10::optional<at::Tensor>& targets, const c10::optional<at::Tensor>& select, int64_t top_k,
-    int64_t n_classes, bool with_stats) {
+using Maybe = c10::optional<at::Tensor>;
+using Scores = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;  // logprob, entropy, top_logprob, top_token
+
+// stats: where the gradient's row statistics go, or nullptr
+Scores scores_of(const at::Tensor& logits, const RowInputs& in, int64_t top_k, int64_t n_classes, at::Tensor* stats) {
   const int dt = dtype_of(logits, "logits");
-  TORCH_CHECK(logits.dim() >= 1 && n_classes >= 1 && n_classes <= logits.size(-1), "evodiff_amd: n_classes must be in [1, ", logits.dim() ? logits.size(-1) : 0, "], got ", n_classes);
-  TORCH_CHECK(top_k >= 0 && top_k <= n_classes && top_k <= ED_TOP_K_MAX, "evodiff_amd: top_k must be in [0, min(n_classes, ", ED_TOP_K_MAX, ")], got ", top_k);
-  const c10::DeviceGuard guard(logits.device());
-  const RowInputs in = row_inputs(logits, targets, select);
   const LogitRows r = logit_rows(logits);
   std::vector<int64_t> shape = logits.sizes().vec();
   shape.pop_back();
   const auto f32 = logits.options().dtype(at::kFloat);
-  at::Tensor logprob = targets.has_value() ? at::empty(shape, f32) : at::empty({0}, f32);
+  at::Tensor logprob = in.targets.has_value() ? at::empty(shape, f32) : at::empty({0}, f32);
   at::Tensor entropy = at::empty(shape, f32);
-  at::Tensor stats = at::empty({with_stats ? r.rows : 0, 2}, f32);
+  if (stats) *stats = at::empty({r.rows, 2}, f32);
   shape.push_back(top_k);
   at::Tensor top = at::empty(shape, f32), token = at::empty(shape, f32.dtype(at::kLong));
   const int64_t need = ed_token_logprobs_workspace(r.rows, n_classes, (int)top_k);
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, f32.dtype(at::kByte));
   check(ed_token_logprobs(r.t.data_ptr(), dt, r.row_stride, r.inner, r.outer_stride, r.rows, n_classes, ptr_or_null<int64_t>(in.targets),
-                          ptr_or_null<uint8_t>(in.select), (int)top_k, targets.has_value() ? logprob.data_ptr<float>() : nullptr,
-                          entropy.data_ptr<float>(), with_stats ? stats.data_ptr<float>() : nullptr, top.data_ptr<float>(),
+                          ptr_or_null<uint8_t>(in.select), (int)top_k, in.targets.has_value() ? logprob.data_ptr<float>() : nullptr,
+                          entropy.data_ptr<float>(), stats ? stats->data_ptr<float>() : nullptr, top.data_ptr<float>(),
                           token.data_ptr<int64_t>(), need > 0 ? ws.data_ptr() : nullptr, need, current_stream(logits)));
-  return {logprob, entropy, top, token, stats};
+  return {logprob, entropy, top, token};
 }
 
-at::Tensor token_logprobs_backward(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
-                                   const c10::optional<at::Tensor>& select, int64_t top_k, int64_t n_classes,
-                                   const at::Tensor& stats, const at::Tensor& entropy, const at::Tensor& top_token,
-                                   const c10::optional<at::Tensor>& g_logprob, const c10::optional<at::Tensor>& g_entropy,
-                                   const c10::optional<at::Tensor>& g_top) {
-  const int dt = dtype_of(logits, "logits");
-  TORCH_CHECK(logits.dim() >= 1 && n_classes >= 1 && n_classes <= logits.size(-1), "evodiff_amd: n_classes must be in [1, V]");
-  TORCH_CHECK(top_k >= 0 && top_k <= n_classes && top_k <= ED_TOP_K_MAX, "evodiff_amd: top_k out of range");
+RowInputs checked_inputs(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
+  dtype_of(logits, "logits");
+  TORCH_CHECK(logits.dim() >= 1 && n_classes >= 1 && n_classes <= logits.size(-1), "evodiff_amd: n_classes must be in [1, ", logits.dim() ? logits.size(-1) : 0, "], got ", n_classes);
+  TORCH_CHECK(top_k >= 0 && top_k <= n_classes && top_k <= ED_TOP_K_MAX, "evodiff_amd: top_k must be in [0, min(n_classes, ", ED_TOP_K_MAX, ")], got ", top_k);
+  return row_inputs(logits, targets, select);
+}
+
+Scores token_logprobs(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
   const c10::DeviceGuard guard(logits.device());
-  const RowInputs in = row_inputs(logits, targets, select);
+  return scores_of(logits, checked_inputs(logits, targets, select, top_k, n_classes), top_k, n_classes, nullptr);
+}
+
+at::Tensor grad_of(const at::Tensor& logits, const RowInputs& in, int64_t top_k, int64_t n_classes, const at::Tensor& stats,
+                   const at::Tensor& entropy, const at::Tensor& top_token, const at::Tensor (&grads)[3]) {
   const LogitRows r = logit_rows(logits);
-  want(stats, at::kFloat, "row_stats");
-  want(entropy, at::kFloat, "entropy");
-  want(top_token, at::kLong, "top_token");
-  same_device(logits, stats, "row_stats");
-  same_device(logits, entropy, "entropy");
-  same_device(logits, top_token, "top_token");
-  TORCH_CHECK(stats.numel() == 2 * r.rows && entropy.numel() == r.rows && top_token.numel() == r.rows * top_k, "evodiff_amd: row_stats, entropy and top_token must be those of the forward call");
-  c10::optional<at::Tensor> g[3];
-  const c10::optional<at::Tensor>* given[3] = {&g_logprob, &g_entropy, &g_top};
-  for (int i = 0; i < 3; ++i)
-    if (given[i]->has_value()) {
-      const at::Tensor& t = **given[i];
-      TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.numel() == r.rows * (i == 2 ? top_k : 1), "evodiff_amd: gradients must be fp32 of the outputs' shapes");
-      same_device(logits, t, "a gradient");
-      g[i] = t.contiguous();
-    }
+  at::Tensor g[3];
+  const float* p[3] = {nullptr, nullptr, nullptr};
+  for (int i = 0; i < 3; ++i) {
+    if (!grads[i].defined() || (i == 0 && !in.targets.has_value()) || (i == 2 && top_k == 0)) continue;
+    TORCH_CHECK(grads[i].is_cuda() && grads[i].numel() == r.rows * (i == 2 ? top_k : 1), "evodiff_amd: gradients must have the outputs' shapes");
+    same_device(logits, grads[i], "a gradient");
+    g[i] = grads[i].to(at::kFloat).contiguous();
+    p[i] = g[i].data_ptr<float>();
+  }
   at::Tensor grad = at::empty(logits.sizes(), logits.options());
-  check(ed_token_logprobs_backward(r.t.data_ptr(), dt, r.row_stride, r.inner, r.outer_stride, r.rows, n_classes, logits.size(-1),
-                                   ptr_or_null<int64_t>(in.targets), ptr_or_null<uint8_t>(in.select), (int)top_k,
-                                   stats.data_ptr<float>(), entropy.data_ptr<float>(), top_token.data_ptr<int64_t>(),
-                                   ptr_or_null<float>(g[0]), ptr_or_null<float>(g[1]), ptr_or_null<float>(g[2]), grad.data_ptr(),
-                                   current_stream(logits)));
+  check(ed_token_logprobs_backward(r.t.data_ptr(), dtype_of(logits, "logits"), r.row_stride, r.inner, r.outer_stride, r.rows, n_classes,
+                                   logits.size(-1), ptr_or_null<int64_t>(in.targets), ptr_or_null<uint8_t>(in.select), (int)top_k,
+                                   stats.data_ptr<float>(), entropy.data_ptr<float>(), top_token.data_ptr<int64_t>(), p[0], p[1], p[2],
+                                   grad.data_ptr(), current_stream(logits)));
   return grad;
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const Maybe& targets,
+                                                const Maybe& select, int64_t top_k, int64_t n_classes) {
+    const at::AutoDispatchBelowAutograd below;
+    const c10::DeviceGuard guard(logits.device());
+    const RowInputs in = checked_inputs(logits, targets, select, top_k, n_classes);
+    at::Tensor stats;
+    const Scores out = scores_of(logits, in, top_k, n_classes, &stats);
+    ctx->save_for_backward({logits, in.targets.value_or(at::Tensor()), in.select.value_or(at::Tensor()), stats, std::get<1>(out), std::get<3>(out)});
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["n_classes"] = n_classes;
+    ctx->mark_non_differentiable({std::get<3>(out)});
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const at::Tensor& logits = saved[0];
+    at::Tensor grad;
+    {
+      const at::AutoDispatchBelowAutograd below;
+      const c10::DeviceGuard guard(logits.device());
+      RowInputs in;
+      if (saved[1].defined()) in.targets = saved[1];
+      if (saved[2].defined()) in.select = saved[2];
+      const at::Tensor given[3] = {grads[0], grads[1], grads[2]};
+      grad = grad_of(logits, in, ctx->saved_data["top_k"].toInt(), ctx->saved_data["n_classes"].toInt(), saved[3], saved[4], saved[5], given);
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: the gradient itself has none, and says so where one is asked for
+      const auto once = std::make_shared<torch::autograd::DelayedError>("token_logprobs can be differentiated once only", 1);
+      grad = (*once)({grad.detach().requires_grad_()})[0];
+    }
+    return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+Scores token_logprobs_autograd(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    const at::AutoDispatchBelowAutograd below;
+    return token_logprobs(logits, targets, select, top_k, n_classes);
+  }
+  const auto out = TokenLogprobs::apply(logits, targets, select, top_k, n_classes);
+  return {out[0], out[1], out[2], out[3]};
 }
 
 }  // namespace
@@ -331,8 +372,7 @@ TORCH_LIBRARY(evodiff_amd, m) {
   m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)");
   m.def("quantize_fp8_weight(Tensor w) -> (Tensor, Tensor)");
   m.def("linear_fp8(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType? out_dtype) -> Tensor");
-  m.def("token_logprobs(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes, bool with_stats) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def("token_logprobs_backward(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes, Tensor row_stats, Tensor entropy, Tensor top_token, Tensor? grad_logprob, Tensor? grad_entropy, Tensor? grad_top) -> Tensor");
+  m.def("token_logprobs(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(evodiff_amd, CUDA, m) {
@@ -344,5 +384,8 @@ TORCH_LIBRARY_IMPL(evodiff_amd, CUDA, m) {
   m.impl("quantize_fp8_weight", &quantize_fp8_weight);
   m.impl("linear_fp8", &linear_fp8);
   m.impl("token_logprobs", &token_logprobs);
-  m.impl("token_logprobs_backward", &token_logprobs_backward);
+}
+
+TORCH_LIBRARY_IMPL(evodiff_amd, AutogradCUDA, m) {
+  m.impl("token_logprobs", &token_logprobs_autograd);
 }

@@ -19,8 +19,6 @@ import torch
 from . import torch_ops
 from ._lib import EvoDiffHipError
 
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
-
 
 class Fp8Rows(NamedTuple):
     """Rows in 8 bits: ``q`` (rows, Kb * 128) float8_e4m3fn, ``scale`` (rows, Kb) float8_e8m0fnu, Kb = ceil(K / 128)."""
@@ -43,25 +41,22 @@ class TokenLogprobs(NamedTuple):
     top_token: torch.Tensor
 
 
-def _on_gpu(*tensors):
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise EvoDiffHipError("evodiff_amd has no CPU path: move the inputs to the GPU")
-    if len({t.device for t in tensors if t is not None}) > 1:
-        raise ValueError("all tensors of a call must be on one device")
+def _on_gpu(t):
+    if not t.is_cuda:
+        raise EvoDiffHipError("evodiff_amd has no CPU path: move the inputs to the GPU")
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """``x`` (..., K) fp32 / bf16 / fp16 -> rows in 8 bits, a scale for 128 channels of a row (leading dimensions are
     flattened).  Rounded to nearest even; infinities and NaN become NaN."""
     _on_gpu(x)
-    return Fp8Rows(*torch_ops.load().quantize_fp8(x.detach()))
+    return Fp8Rows(*torch_ops.load().quantize_fp8(x.detach() if x.requires_grad else x))
 
 
 def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
     """``w`` (N, K) fp32 / bf16 / fp16 -> a weight in 8 bits, one scale for 128 x 128 values."""
     _on_gpu(w)
-    return Fp8Weight(*torch_ops.load().quantize_fp8_weight(w.detach()))
+    return Fp8Weight(*torch_ops.load().quantize_fp8_weight(w.detach() if w.requires_grad else w))
 
 
 def linear_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optional[torch.Tensor] = None,
@@ -71,31 +66,12 @@ def linear_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optiona
     share.  ``weight``: from ``quantize_fp8_weight``.  ``bias``: fp32 (N,).  ``out_dtype``: that of ``x`` by default (bf16 for
     ``Fp8Rows``).  An operator of inference: it has no gradient, and refuses an ``x`` or ``bias`` that asks for one."""
     rows, scale = (x.q, x.scale) if isinstance(x, Fp8Rows) else (x, None)
-    _on_gpu(rows, scale, weight.q, weight.scale, bias)
+    _on_gpu(rows)
     if torch.is_grad_enabled() and (rows.requires_grad or (bias is not None and bias.requires_grad)):
         raise EvoDiffHipError("linear_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    if rows.requires_grad:
+        rows = rows.detach()
     return torch_ops.load().linear_fp8(rows, scale, weight.q, weight.scale, bias, out_dtype)
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, select, top_k, n_classes):
-        logprob, entropy, top_logprob, top_token, stats = torch_ops.load().token_logprobs(logits, targets, select, top_k,
-                                                                                          n_classes, True)
-        ctx.save_for_backward(logits, targets, select, stats, entropy, top_token)
-        ctx.top_k, ctx.n_classes = top_k, n_classes
-        ctx.mark_non_differentiable(top_token)
-        ctx.set_materialize_grads(False)
-        return logprob, entropy, top_logprob, top_token
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_top, _):
-        logits, targets, select, stats, entropy, top_token = ctx.saved_tensors
-        grad = torch_ops.load().token_logprobs_backward(logits, targets, select, ctx.top_k, ctx.n_classes, stats, entropy,
-                                                        top_token, g_logprob if targets is not None else None, g_entropy,
-                                                        g_top)
-        return grad, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top_k: int = 0,
@@ -110,12 +86,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top_k:
     strided leading dimensions (``logits[:, :-1]``); others are copied first.
 
     Differentiable once in ``logprob``, ``entropy`` and ``top_logprob``."""
-    _on_gpu(logits, targets, select)
-    if logits.dim() < 1:
-        raise ValueError("logits must have a dimension of classes")
-    n_classes = logits.shape[-1] if n_classes is None else int(n_classes)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        out = _TokenLogprobs.apply(logits, targets, select, int(top_k), n_classes)
-    else:
-        out = torch_ops.load().token_logprobs(logits.detach(), targets, select, int(top_k), n_classes, False)[:4]
+    _on_gpu(logits)
+    n_classes = (logits.shape[-1] if logits.dim() else 0) if n_classes is None else int(n_classes)
+    out = torch_ops.load().token_logprobs(logits, targets, select, top_k, n_classes)
     return TokenLogprobs(out[0] if targets is not None else None, *out[1:])

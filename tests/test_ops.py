@@ -545,6 +545,26 @@ def test_gradient_against_differences(dev, v):
 
 
 @gpu
+def test_gradient_is_taken_once_and_in_any_grad_mode(dev):
+    x = rand(dev, (4, 31), 0).requires_grad_()
+    t = torch.zeros(4, dtype=torch.long, device=dev)
+    grad, = torch.autograd.grad(ops.token_logprobs(x, t).logprob.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grad.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        grad.sum().backward()
+    want, = torch.autograd.grad(ops.token_logprobs(x, t).logprob.sum(), x)
+    assert torch.equal(grad, want)
+    with torch.no_grad():
+        assert not ops.token_logprobs(x, t).logprob.requires_grad
+    assert not ops.token_logprobs(x.detach(), t).logprob.requires_grad
+    out = ops.token_logprobs(x, t, 3)
+    assert out.entropy.requires_grad and out.top_logprob.requires_grad and not out.top_token.requires_grad
+    out.entropy.mean().backward()
+    assert x.grad is not None and x.grad.shape == x.shape
+
+
+@gpu
 def test_gradient_of_views_classes_broadcast_and_missing_targets(dev):
     v = 40
     base = rand(dev, (3, 5, v), 1).requires_grad_()
