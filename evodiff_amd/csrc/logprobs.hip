@@ -614,8 +614,13 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
       const int s = i / top_k;
       keys[i] = ((const u64*)(src + s * piece_bytes(top_k) + sizeof(Piece)))[i - s * top_k];
     }
-    Sums2 a = ((const Piece*)src)->sums;
-    for (int s = 1; s < splits; ++s) a.join(((const Piece*)(src + s * piece_bytes(top_k)))->sums);
+    Sums2 a{NEG_INF, R_MIN, 0.f, 0.f};  // every wave joins all pieces, one a lane
+    if ((tid & 63) < splits) a = ((const Piece*)(src + (tid & 63) * piece_bytes(top_k)))->sums;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const Sums2 b{__shfl_xor(a.m, o), __shfl_xor(a.r, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
+      a.join(b);
+    }
     const bool plain = (a.m > PLAIN_FROM || a.m < -PLAIN_FROM) && a.m != NEG_INF;
     const RowEnd res = plain ? RowEnd(plain_sums<DT>(row, x.n, plain_space, tid)) : RowEnd(a);
     if (tid == 0) {
@@ -686,55 +691,108 @@ __device__ __forceinline__ float named(const int64_t* targets, int top_k, const 
   return d;
 }
 
-// A workgroup per tile of 2048 / 4096 classes of a row: four 16-byte loads and stores a thread, where source and destination
-// rows lie alike within 16 bytes; class by class elsewhere.
+// A workgroup per `per` tiles of 256 vectors of a row: 16-byte loads, the next tile's in flight, and 16-byte stores where source
+// and destination rows lie alike within 16 bytes; class by class elsewhere.  The named classes of the piece are listed in
+// shared memory while the first loads fly.
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const int64_t* __restrict__ targets,
                                                             const uint8_t* __restrict__ select, int top_k,
-                                                            LogprobsGrad g, int tiles) {
+                                                            LogprobsGrad g, int pieces, int per) {
   typedef typename Elem<DT>::T T;
-  constexpr int EPV = 16 / sizeof(T), U = 2, TILE = 256 * U * EPV;
+  constexpr int EPV = 16 / sizeof(T), U = 2;
   typedef __attribute__((ext_vector_type(EPV))) T VT;
+  __shared__ int name_at[TOP_MAX + 1];
+  __shared__ float name_add[TOP_MAX + 1];
+  __shared__ int n_names;
   const int tid = threadIdx.x;
-  const long items = x.rows * tiles;
+  const long items = x.rows * pieces;
   for (long item = blockIdx.x; item < items; item += gridDim.x) {
-    const long r = item / tiles;
-    const int tile = (int)(item - r * tiles);
+    const long r = item / pieces;
+    const int piece = (int)(item - r * pieces);
     const T* row = row_of<T>(x, r);
     T* dst = (T*)g.dlogits + r * g.columns;
-    const GradRow a = grad_row(x, targets, select, top_k, g, r);
     const int head = (int)((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / (int)sizeof(T);
     const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
-    // this tile's columns: vectors are counted from the first aligned column, tile 0 also holds the ones in front
-    const long from = tile == 0 ? 0 : head + (long)tile * TILE, end = head + (long)(tile + 1) * TILE;
-    const long to = end < g.columns ? end : g.columns;
-    if (a.skip) {
-      for (long v = from + tid; v < to; v += 256) dst[v] = Elem<DT>::put(0.f);
-      continue;
+    // the vectors of this piece, all of them classes; columns beside vectors are the first and the last piece's
+    const int vectors = alike && x.n > head ? (x.n - head) / EPV : 0;
+    const int v0 = piece * per * 256 < vectors ? piece * per * 256 : vectors;
+    const int v1 = v0 + per * 256 < vectors && piece + 1 < pieces ? v0 + per * 256 : vectors;
+    uint4 next[U];
+    auto load = [&](int at) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (at + u * 256 + tid < v1) next[u] = *(const uint4*)(row + head + (long)(at + u * 256 + tid) * EPV);
+    };
+    load(v0);
+    const GradRow a = grad_row(x, targets, select, top_k, g, r);
+    __syncthreads();
+    if (tid == 0) n_names = 0;
+    __syncthreads();
+    const int has_target = g.g_logprob ? 1 : 0, names = has_target + (g.g_top ? top_k : 0);
+    if (tid < names) {
+      const int64_t v = has_target && tid == 0 ? targets[r] : g.top_token[r * top_k + tid - has_target];
+      if (v >= 0 && v < x.n) {
+        const int64_t vec = (v - head) / EPV;
+        const bool inside = v >= head && vec < vectors;
+        if (inside ? vec >= v0 && vec < v1 : true) {
+          const int slot = atomicAdd(&n_names, 1);  // (a class named twice is listed twice, with the same sum)
+          name_at[slot] = (int)v;
+          name_add[slot] = named(targets, top_k, g, r, v);
+        }
+      }
     }
-    if (alike && from + (tile == 0 ? head : 0) + TILE <= x.n) {
+    __syncthreads();
+    const int listed = n_names;
+    for (int at = v0; at < v1; at += 256 * U) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      load(at + 256 * U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const long v = head + (long)tile * TILE + (u * 256 + tid) * EPV;
-        const uint4 raw = *(const uint4*)(row + v);
+        const int vec = at + u * 256 + tid;
+        if (vec >= v1) continue;
+        const int first = head + vec * EPV;
         float f[EPV];
-        unpack<DT>(raw, f);
+        unpack<DT>(raw[u], f);
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) f[i] = a.at(f[i]);
+        for (int j = 0; j < listed; ++j) {
+          const int off = name_at[j] - first;
+          if (off >= 0 && off < EPV) {
+            bool again = false;
+            for (int k = 0; k < j; ++k) again |= name_at[k] == name_at[j];
+            if (!again) {
+#pragma unroll
+              for (int i = 0; i < EPV; ++i) f[i] += off == i ? name_add[j] : 0.f;
+            }
+          }
+        }
         VT o;
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) o[i] = Elem<DT>::put(a.at(f[i]));
-        *(VT*)(dst + v) = o;
+        for (int i = 0; i < EPV; ++i) o[i] = Elem<DT>::put(a.skip ? 0.f : f[i]);
+        *(VT*)(dst + first) = o;
       }
-      if (tile == 0 && tid < head) dst[tid] = Elem<DT>::put(a.at(Elem<DT>::get(row[tid])));
-    } else {
-      for (long v = from + tid; v < to; v += 256) dst[v] = Elem<DT>::put(v < x.n ? a.at(Elem<DT>::get(row[v])) : 0.f);
     }
-    const int names = (g.g_logprob ? 1 : 0) + (g.g_top ? top_k : 0);
-    if (names) {
-      __syncthreads();  // (also waits for the stores above)
-      if (tid < names) {
-        const int64_t v = g.g_logprob && tid == 0 ? targets[r] : g.top_token[r * top_k + tid - (g.g_logprob ? 1 : 0)];
-        if (v >= from && v < to && v < x.n) dst[v] = Elem<DT>::put(a.at(Elem<DT>::get(row[v])) + named(targets, top_k, g, r, v));
+    auto one = [&](long v) {
+      float d = 0.f;
+      if (!a.skip && v < x.n) {
+        d = a.at(Elem<DT>::get(row[v]));
+        for (int j = 0; j < listed; ++j)
+          if (name_at[j] == v) {
+            d += name_add[j];
+            break;
+          }
       }
+      dst[v] = Elem<DT>::put(d);
+    };
+    if (vectors > 0) {
+      if (piece == 0 && tid < head) one(tid);
+      if (piece + 1 == pieces)
+        for (long v = head + (long)vectors * EPV + tid; v < g.columns; v += 256) one(v);
+    } else {
+      const long span = (g.columns + pieces - 1) / pieces, to = (piece + 1) * span < g.columns ? (piece + 1) * span : g.columns;
+      for (long v = piece * span + tid; v < to; v += 256) one(v);
     }
   }
 }
@@ -817,9 +875,13 @@ static hipError_t launch_grad(const LogitsView& x, const int64_t* targets, const
     hipLaunchKernelGGL((logprobs_grad_flat_kernel<DT>), blocks((x.rows * g.columns + 255) / 256), dim3(256), 0, stream, x, targets,
                        select, top_k, g);
   } else {
-    const long tile = 256 * 2 * (16 / dt_bytes(DT));
-    const int tiles = (int)((g.columns + tile - 1) / tile);  // (the columns in front of the first aligned one are tile 0's)
-    hipLaunchKernelGGL((logprobs_grad_kernel<DT>), blocks(x.rows * tiles), dim3(256), 0, stream, x, targets, select, top_k, g, tiles);
+    // tiles of 256 vectors in a workgroup: eight where the rows are many (the row's scalars and names are read once for
+    // them), down to two so that few rows still fill the chip eight workgroups a CU deep
+    const long tiles = (g.columns / (16 / dt_bytes(DT)) + 255) / 256;
+    int per = 8;
+    while (per > 2 && x.rows * ((tiles + per - 1) / per) < 2048) per /= 2;
+    const int pieces = (int)((tiles + per - 1) / per);
+    hipLaunchKernelGGL((logprobs_grad_kernel<DT>), blocks(x.rows * pieces), dim3(256), 0, stream, x, targets, select, top_k, g, pieces, per);
   }
   return hipGetLastError();
 }
