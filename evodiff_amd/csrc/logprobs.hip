@@ -299,9 +299,9 @@ __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[16 / sizeof(
 }
 
 struct TopSpace {
-  u64 best[256];               // a thread's best group
+  alignas(16) u64 best[256];   // a thread's best group
   u64 list[LIST];              // groups that reached tau
-  u64 found[GROUPS * 8];       // classes that may be among the k
+  alignas(16) u64 found[GROUPS * 8 + 8];  // classes that may be among the k, zeros up to a multiple of eight
   int group[GROUPS];
   u64 tau;
   int listed, groups, n_found;
@@ -317,19 +317,30 @@ __device__ __forceinline__ void renew_tau(TopSpace& sp, u64 mine, int top_k, int
     __builtin_amdgcn_wave_barrier();
     int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < 64; ++j) rank += sp.best[j] > k;
+    for (int j = 0; j < 64; j += 2) {
+      const ulonglong2 two = *(const ulonglong2*)(sp.best + j);
+      rank += (two.x > k) + (two.y > k);
+    }
     if (rank == top_k - 1 && k) sp.tau = k;
   }
   __syncthreads();
 }
 
-// out[rank] = the k largest of sp.found[0 .. n) in order, by counting; n >= k
+// put(rank, key) for the k largest of found[0 .. n), by counting; found holds eight more (16-byte aligned).  A barrier is inside.
 template <typename Put>
-__device__ __forceinline__ void rank_found(const u64* found, int n, int top_k, int tid, Put put) {
+__device__ __forceinline__ void rank_found(u64* found, int n, int top_k, int tid, Put put) {
+  if (tid < 8) found[n + tid] = 0;
+  __syncthreads();
   for (int i = tid; i < n; i += 256) {
     const u64 k = found[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += found[j] > k;
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const ulonglong2 two = *(const ulonglong2*)(found + j + e);
+        rank += (two.x > k) + (two.y > k);
+      }
+    }
     if (rank < top_k) put(rank, k);
   }
 }
@@ -391,7 +402,7 @@ struct Piece {  // of a row: its sums, followed in memory by top_k keys
 __host__ __device__ inline long piece_bytes(int top_k) { return (long)sizeof(Piece) + 8L * top_k; }
 
 template <int DT, bool TOP>
-__global__ __launch_bounds__(256) void logprobs_stream_kernel(LogitsView x, const int64_t* __restrict__ targets,
+__global__ __launch_bounds__(256, 5) void logprobs_stream_kernel(LogitsView x, const int64_t* __restrict__ targets,
                                                               const uint8_t* __restrict__ select, int top_k,
                                                               LogprobsOut out, char* __restrict__ pieces, int splits) {
   typedef typename Elem<DT>::T T;
@@ -464,19 +475,14 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(LogitsView x, cons
       for (int u = 0; u < U; ++u) raw[u] = next[u];
       load(next, at + 256 * U);
       float high[U];
-      float v[EPV];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        float v[EPV];
         unpack<DT>(raw[u], v);
         high[u] = v[0];
 #pragma unroll
         for (int i = 1; i < EPV; ++i) high[u] = fmaxf(high[u], v[i]);
-      }
-      const float top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
-      if (__any(top > a.m)) raise(top);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        unpack<DT>(raw[u], v);
+        if (__any(high[u] > a.m)) raise(high[u]);
 #pragma unroll
         for (int i = 0; i < EPV; ++i) add(v[i]);
       }
@@ -495,7 +501,7 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(LogitsView x, cons
           tau_value = tau ? key_value(tau) : NEG_INF;
           renew_at *= 2;
         }
-        if (__any(top >= tau_value)) {
+        if (__any(fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) >= tau_value)) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int g = at + u * 256 + tid;
@@ -593,7 +599,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
                                                             const char* __restrict__ pieces, int splits) {
   typedef typename Elem<DT>::T T;
   __shared__ u64 keys[64 * TOP_MAX];
-  __shared__ u64 found[64 * TOP_MAX];
+  __shared__ alignas(16) u64 found[64 * TOP_MAX + 8];
   __shared__ u64 tau;
   __shared__ int n_found;
   __shared__ float plain_space[768];
