@@ -8,6 +8,8 @@
 
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 namespace ed {
 namespace {
 
@@ -65,16 +67,14 @@ __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
   return r;
 }
 
-// 16 lanes own a block of 128.
-template <int DT>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, long row_stride, long blocks,
-                                                            int kb, long K, bool wide, uint8_t* __restrict__ q,
-                                                            uint8_t* __restrict__ scale) {
-  const long blk = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (blk >= blocks) return;
-  const int l = threadIdx.x & 15;
-  const long row = blk / kb;
-  const int b = (int)(blk - row * kb);
+// 16 lanes own a block of 128; the 16 blocks of a workgroup are the same channels of 16 rows.  TURNED: scales go to (kb, rows),
+// as the product reads them (16 rows' bytes side by side), instead of (rows, kb).
+template <int DT, bool TURNED>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, long row_stride, long rows, int kb, long K,
+                                                            bool wide, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  const long row = blockIdx.x / kb * 16 + (threadIdx.x >> 4);
+  const int b = (int)(blockIdx.x % kb), l = threadIdx.x & 15;
+  if (row >= rows) return;
   float v[8];
   load8<DT>((const typename Elem<DT>::T*)x + row * row_stride, (long)b * FP8_BLOCK + l * 8, K, wide, v);
   unsigned a = amax8(v);
@@ -84,8 +84,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
     a = c > a ? c : a;
   }
   const int byte = scale_byte(a);
-  *(uint2*)(q + blk * FP8_BLOCK + l * 8) = pack8(v, inverse_scale(byte));
-  if (l == 0) scale[blk] = (uint8_t)byte;
+  *(uint2*)(q + (row * kb + b) * FP8_BLOCK + l * 8) = pack8(v, inverse_scale(byte));
+  if (l == 0) scale[TURNED ? b * rows + row : row * kb + b] = (uint8_t)byte;
 }
 
 // One workgroup per 128 x 128 weights: thread (r, c) holds columns 8c .. 8c + 7 of rows r, r + 16, ...
@@ -127,16 +127,6 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
   if (threadIdx.x == 0) scale[nb * kb + b] = (uint8_t)byte;
 }
 
-template <int OUT_DT>
-__device__ __forceinline__ void store_out(void* out, long at, float v) {
-  ((typename Elem<OUT_DT>::T*)out)[at] = (typename Elem<OUT_DT>::T)v;
-}
-
-// 16 bytes of K at chunk c (of 8) of a block row
-__device__ __forceinline__ i32x8 load_fragment(const uint8_t* row, int fq) {
-  const i32x4 a = *(const i32x4*)(row + fq * 16), b = *(const i32x4*)(row + 64 + fq * 16);
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
 
 // Eight products at a time, the 8-bit matrix instructions (scaled or not, any shape) align to the largest and drop what lies
 // under 2^-13 of it: results are 4e-5 to 6e-5 (2-norm) from the exact sum at any K, well under half a step of bf16 (2e-3) or fp16
@@ -160,8 +150,204 @@ __device__ __forceinline__ float scale_of(int byte) {  // 2^(byte - 127)
   return byte == 0 ? __uint_as_float(0x400000u) : byte == 255 ? __builtin_nanf("") : __uint_as_float((unsigned)byte << 23);
 }
 
-// A wave per 32 x 32 results, operands straight from memory.  The weights are the instruction's row operand: a lane then
-// holds four consecutive channels of one row.  Rows and channels past the end read the last one and are not stored.
+__device__ __forceinline__ void copy16(const uint8_t* src, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Tiled product.  Four waves, 2 (rows) x 2 (channels), own a tile of 32 WTM rows x 32 WTN channels, a wave 16 WTM x 16 WTN as
+// WTN x WTM instructions of 16 x 16 x 128: one per block of K and pair of fragments, its scales beside it.
+//
+// Step of K (one block): rows of 128 bytes of both operands, copied memory -> LDS a step ahead into one of two stages.  The
+// 16-byte chunk c of tile row r lies at chunk c ^ (r >> 1 & 7) (the copy's source addresses are permuted, its image is
+// lane-linear): the 16 rows of a fragment read then fall on 16 different slots of the banks.
+//
+// Order inside a step.  A wave's channel fragments pass through a ring of four, its row fragments stay for the step.  Once
+// the last channel fragment of the step is read (row of instructions JB), the one barrier of the step: behind it the next
+// stage has landed and this one is free.  The rows of instructions left cover the reads of the next step's first fragments and
+// the copies of the step after, so that neither the barrier nor a read leaves the matrix pipe without work.  The
+// order is pinned (sched_barrier): at most two auxiliary instructions behind each matrix instruction.
+//
+// The channels of an LDS tile are permuted within 32 so that two instructions give a lane eight consecutive ones: 16-byte stores.
+// ---------------------------------------------------------------------------------------------------
+template <int WTM, int WTN, int OUT_DT>
+__global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
+  constexpr int BM = 32 * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
+  constexpr int GX = BM / 32, GW = BN / 32, NG = GX + GW;  // 8-row copies a wave makes of each operand
+  constexpr int RING = 4, JB = WTN > 4 ? WTN - 3 : WTN - 2;  // the barrier stands before row JB of instructions
+  static_assert(JB >= WTN - RING + 1 && JB >= 1, "every channel fragment of a step is read in front of its barrier");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4, wr = wid >> 1, wc = wid & 1;
+
+  // Tiles: workgroups id, id + 8, ... share an XCD and its L2; each XCD takes a run of the order in which four tile rows are
+  // walked column by column, so that what it holds at a time is a compact block.
+  int tile_m, tile_n;
+  {
+    const int total = tiles_m * tiles_n, id = blockIdx.x, q = total >> 3, r = total & 7, xcd = id & 7;
+    const int at = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+    const int per = 4 * tiles_n, band = at / per, in = at - band * per, high = min(tiles_m - 4 * band, 4);
+    tile_n = in / high;
+    tile_m = 4 * band + in - tile_n * high;
+  }
+  const long m0 = (long)tile_m * BM, n0 = (long)tile_n * BN, pitch = (long)g.kb * FP8_BLOCK;
+  const int T = g.kb;
+
+  // copies: lane -> (row of 8, physical chunk); rows past the end repeat the last one
+  const int chunk0 = ((lane & 7) ^ (lane >> 4)) * 16, chunk1 = ((lane & 7) ^ (4 + (lane >> 4))) * 16;
+  unsigned off[NG];
+#pragma unroll
+  for (int j = 0; j < GX; ++j) {
+    const int row = (wid * GX + j) * 8 + (lane >> 3), left = (int)(g.M - 1 - m0 < BM ? g.M - 1 - m0 : BM);
+    off[j] = (unsigned)((row < left ? row : left) * pitch) + ((wid * GX + j) & 1 ? chunk1 : chunk0);
+  }
+#pragma unroll
+  for (int j = 0; j < GW; ++j) {
+    const int lr = (wid * GW + j) * 8 + (lane >> 3), left = (int)(g.N - 1 - n0 < BN ? g.N - 1 - n0 : BN);
+    const int ch = (lr & ~31) + 8 * ((lr & 15) >> 2) + 4 * ((lr >> 4) & 1) + (lr & 3);
+    off[GX + j] = (unsigned)((ch < left ? ch : left) * pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
+  }
+  const uint8_t* x_src = g.xq + m0 * pitch;
+  const uint8_t* w_src = g.wq + n0 * pitch;
+  auto copy = [&](int j, char* stage) {  // piece j of the step that x_src and w_src stand at
+    if (j < GX) copy16(x_src + off[j], stage + (wid * GX + j) * 1024);
+    else copy16(w_src + off[j], stage + BM * 128 + (wid * GW + j - GX) * 1024);
+  };
+
+  // scales: a lane's row in each of the WTM fragments; the wave's channels lie in one block of 128
+  unsigned sx_off[WTM];
+#pragma unroll
+  for (int i = 0; i < WTM; ++i) {
+    const long m = m0 + wr * 16 * WTM + i * 16 + fr;
+    sx_off[i] = (unsigned)(m < g.M ? m : g.M - 1);
+  }
+  const long nw = n0 + wc * 16 * WTN;
+  const uint8_t* sw_src = g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb;
+  const uint8_t* sx_src = g.xs;  // (kb, M)
+
+  const int swz = (fq ^ ((fr >> 1) & 7)) << 4;
+  const int x_rd = (wr * 16 * WTM + fr) * 128, w_rd = BM * 128 + (wc * 16 * WTN + fr) * 128;
+  auto read = [&](const char* stage, int base, int half) { return *(const i32x4*)(stage + base + ((half << 6) ^ swz)); };
+  auto put = [](i32x8& f, int half, i32x4 v) {
+    if (half == 0) { f[0] = v[0]; f[1] = v[1]; f[2] = v[2]; f[3] = v[3]; }
+    else { f[4] = v[0]; f[5] = v[1]; f[6] = v[2]; f[7] = v[3]; }
+  };
+
+  f32x4 acc[WTN][WTM] = {};
+  i32x8 X[WTM], W[RING];
+  int sx[WTM], sx_next[WTM], sw, sw_next;
+
+  // step t = 0 in flight, its first fragments, step 1's copies
+#pragma unroll
+  for (int j = 0; j < NG; ++j) copy(j, lds);
+#pragma unroll
+  for (int i = 0; i < WTM; ++i) sx[i] = sx_src[sx_off[i]];
+  sw = sw_src[0];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WTM; ++i) { put(X[i], 0, read(lds, x_rd + i * 2048, 0)); put(X[i], 1, read(lds, x_rd + i * 2048, 1)); }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) { put(W[j], 0, read(lds, w_rd + j * 2048, 0)); put(W[j], 1, read(lds, w_rd + j * 2048, 1)); }
+  // The copies run two steps ahead; past the last step they repeat its block (in bounds, into a stage nobody reads).
+  int ahead = 0;
+  auto advance = [&]() {
+    const long d = ++ahead < T ? FP8_BLOCK : 0;
+    x_src += d;
+    w_src += d;
+  };
+  advance();
+#pragma unroll
+  for (int j = 0; j < NG; ++j) copy(j, lds + STAGE);
+
+  for (int t = 0; t < T; ++t) {
+    char* const here = lds + (t & 1) * STAGE;
+    const char* const there = lds + (1 - (t & 1)) * STAGE;
+    const int more = t + 1 < T ? 1 : 0;
+    sx_src += more ? g.M : 0;
+    sw_src += more;
+#pragma unroll
+    for (int j = 0; j < WTN; ++j) {
+      if (j == JB) {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();  // (drains this wave's copies and reads)
+        advance();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < WTM; ++i) {
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, sw, 0, sx[i]);
+        const int slot = j * WTM + i;
+        if (j < JB) {
+          // channel fragments 2 .. WTN - 1, two reads each, as soon as their slot of the ring is free
+#pragma unroll
+          for (int r = 0; r < 2 * (WTN - 2); ++r) {
+            const int f = 2 + r / 2, want = f < RING ? r : (f - RING + 1) * WTM + (r & 1);
+            if (want == slot) put(W[f % RING], r & 1, read(here, w_rd + f * 2048, r & 1));
+          }
+          if (slot >= 4 && slot < 4 + WTM) sx_next[slot - 4] = sx_src[sx_off[slot - 4]];  // the next step's scales
+          if (slot == 4) sw_next = sw_src[0];
+        } else {
+          constexpr int COPY_SLOTS = (WTN - JB) * WTM;
+          const int after = slot - JB * WTM;
+#pragma unroll
+          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, here);
+          // the next step's first two channel fragments: slot 0 is free, slot 1 too unless row JB of instructions reads it
+          constexpr int W1_AT = JB % RING == 1 ? WTM : 2;
+          if (after < 2) put(W[0], after, read(there, w_rd, after));
+          if (after >= W1_AT && after < W1_AT + 2) put(W[1], after - W1_AT, read(there, w_rd + 2048, after - W1_AT));
+          if (j == WTN - 1) {
+            put(X[i], 0, read(there, x_rd + i * 2048, 0));  // in place: X[i] has done its last instruction of the step
+            put(X[i], 1, read(there, x_rd + i * 2048, 1));
+            sx[i] = sx_next[i];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    sw = sw_next;
+  }
+  __syncthreads();  // (no copy may land once this workgroup's shared memory is another's)
+
+  // ---- results: acc[2 J][i], acc[2 J + 1][i] are channels nw + 32 J + 8 fq + 0 .. 3, 4 .. 7 of row i * 16 + fr
+  typedef typename Elem<OUT_DT>::T T_out;
+  typedef __attribute__((ext_vector_type(8))) T_out V8;
+  T_out* const out = (T_out*)g.out;
+  const bool wide = (g.N & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+  for (int J = 0; J < WTN / 2; ++J) {
+    const long n = nw + 32 * J + 8 * fq;
+    float b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = g.bias && n + e < g.N ? g.bias[n + e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < WTM; ++i) {
+      const long m = m0 + wr * 16 * WTM + i * 16 + fr;
+      if (m >= g.M) continue;
+      T_out* const to = out + m * g.N + n;
+      if (wide && n + 8 <= g.N) {
+        V8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[e]);
+        *(V8*)to = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < g.N) to[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[e]);
+      }
+    }
+  }
+}
+
+// Any shape, operands straight from memory, a wave per 32 x 32 results; row scales as in the tiled kernel.
+__device__ __forceinline__ i32x8 load_fragment(const uint8_t* row, int fq) {
+  const i32x4 a = *(const i32x4*)(row + fq * 16), b = *(const i32x4*)(row + 64 + fq * 16);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int OUT_DT>
+__device__ __forceinline__ void store_out(void* out, long at, float v) {
+  ((typename Elem<OUT_DT>::T*)out)[at] = (typename Elem<OUT_DT>::T)v;
+}
 template <int OUT_DT>
 __global__ __launch_bounds__(256) void gemm_kernel(Fp8Gemm g) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -184,7 +370,7 @@ __global__ __launch_bounds__(256) void gemm_kernel(Fp8Gemm g) {
       w[i] = load_fragment(g.wq + rn[i] * pitch + (long)b * FP8_BLOCK, fq);
       x[i] = load_fragment(g.xq + rm[i] * pitch + (long)b * FP8_BLOCK, fq);
       sw[i] = g.ws[(rn[i] >> 7) * g.kb + b];
-      sx[i] = g.xs[rm[i] * g.kb + b];
+      sx[i] = g.xs[b * g.M + rm[i]];
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -211,6 +397,15 @@ __global__ __launch_bounds__(256) void gemm_kernel(Fp8Gemm g) {
     }
 }
 
+// scale (rows, kb) -> (kb, rows)
+__global__ __launch_bounds__(256) void turn_scales_kernel(const uint8_t* __restrict__ scale, uint8_t* __restrict__ turned, long rows, int kb) {
+  const long count = rows * kb;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
+    const long b = i / rows;
+    turned[i] = scale[(i - b * rows) * kb + b];
+  }
+}
+
 bool wide_rows(const void* p, int dt, int64_t row_stride) {  // every row starts on eight aligned elements
   const int64_t align = 8 * dt_bytes(dt) < 16 ? 8 * dt_bytes(dt) : 16;
   return (reinterpret_cast<uintptr_t>(p) % align) == 0 && (row_stride * dt_bytes(dt)) % align == 0;
@@ -218,18 +413,22 @@ bool wide_rows(const void* p, int dt, int64_t row_stride) {  // every row starts
 
 }  // namespace
 
-hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q,
-                                    uint8_t* scale, hipStream_t stream) {
+template <bool TURNED>
+static hipError_t quantize_rows(const void* x, int dt, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q, uint8_t* scale,
+                                hipStream_t stream) {
   const int kb = (int)fp8_blocks(K);
-  const long blocks = rows * kb;
-  const dim3 grid((unsigned)((blocks + 15) / 16));
+  const dim3 grid((unsigned)((rows + 15) / 16 * kb));
   const bool wide = wide_rows(x, dt, row_stride);
-#define ED_GO(DT) hipLaunchKernelGGL((quantize_rows_kernel<DT>), grid, dim3(256), 0, stream, x, (long)row_stride, blocks, kb, (long)K, wide, q, scale)
+#define ED_GO(DT) hipLaunchKernelGGL((quantize_rows_kernel<DT, TURNED>), grid, dim3(256), 0, stream, x, (long)row_stride, (long)rows, kb, (long)K, wide, q, scale)
   if (dt == DT_FP32) ED_GO(DT_FP32);
   else if (dt == DT_BF16) ED_GO(DT_BF16);
   else ED_GO(DT_FP16);
 #undef ED_GO
   return hipGetLastError();
+}
+hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q,
+                                    uint8_t* scale, hipStream_t stream) {
+  return quantize_rows<false>(x, dt, row_stride, rows, K, q, scale, stream);
 }
 
 hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride, int64_t N, int64_t K, uint8_t* q,
@@ -245,31 +444,50 @@ hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride,
   return hipGetLastError();
 }
 
-static hipError_t launch_gemm(const Fp8Gemm& g, hipStream_t stream) {
-  const dim3 grid((unsigned)(((g.N + 63) / 64) * ((g.M + 63) / 64)));
-  if (g.out_dt == DT_FP32) hipLaunchKernelGGL((gemm_kernel<DT_FP32>), grid, dim3(256), 0, stream, g);
-  else if (g.out_dt == DT_BF16) hipLaunchKernelGGL((gemm_kernel<DT_BF16>), grid, dim3(256), 0, stream, g);
-  else hipLaunchKernelGGL((gemm_kernel<DT_FP16>), grid, dim3(256), 0, stream, g);
+template <int WTM, int WTN, int OUT_DT>
+static hipError_t launch_tile(const Fp8Gemm& g, hipStream_t stream) {
+  const int tiles_m = (int)((g.M + 32 * WTM - 1) / (32 * WTM)), tiles_n = (int)((g.N + 32 * WTN - 1) / (32 * WTN));
+  hipLaunchKernelGGL((tile_kernel<WTM, WTN, OUT_DT>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0, stream, g, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
-// workspace: the quantised rows, then their scales
+template <int OUT_DT>
+static hipError_t launch_gemm(const Fp8Gemm& g, hipStream_t stream) {
+  if constexpr (OUT_DT != DT_FP32) {
+    const int64_t big = ((g.M + 255) / 256) * ((g.N + 255) / 256);
+    if (big >= 200) return launch_tile<8, 8, OUT_DT>(g, stream);
+    if (g.M > 64) return launch_tile<4, 4, OUT_DT>(g, stream);
+  }
+  const dim3 grid((unsigned)(((g.N + 63) / 64) * ((g.M + 63) / 64)));
+  hipLaunchKernelGGL((gemm_kernel<OUT_DT>), grid, dim3(256), 0, stream, g);
+  return hipGetLastError();
+}
+
+// workspace: the quantised rows (a multiple of 128 bytes), then their scales, (kb, rows)
 int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised) {
-  return quantised ? 0 : M * fp8_blocks(K) * (FP8_BLOCK + 1);
+  return M * fp8_blocks(K) * (quantised ? 1 : FP8_BLOCK + 1);
 }
 
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   const int kb = (int)fp8_blocks(p.K);
-  Fp8Gemm g{(const uint8_t*)p.x, p.x_scale, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
-  if (p.x_dt != DT_E4M3) {
+  const uint8_t* xq = (const uint8_t*)p.x;
+  uint8_t* xs = (uint8_t*)p.workspace;
+  hipError_t e;
+  if (p.x_dt == DT_E4M3) {
+    const long blocks = (p.M * kb + 255) / 256;
+    hipLaunchKernelGGL(turn_scales_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, p.x_scale, xs, (long)p.M, kb);
+    e = hipGetLastError();
+  } else {
     uint8_t* q = (uint8_t*)p.workspace;
-    uint8_t* scale = q + p.M * kb * FP8_BLOCK;
-    const hipError_t e = launch_fp8_quantize_rows(p.x, p.x_dt, p.row_stride, p.M, p.K, q, scale, stream);
-    if (e != hipSuccess) return e;
-    g.xq = q;
-    g.xs = scale;
+    xs = q + p.M * kb * FP8_BLOCK;
+    e = quantize_rows<true>(p.x, p.x_dt, p.row_stride, p.M, p.K, q, xs, stream);
+    xq = q;
   }
-  return launch_gemm(g, stream);
+  if (e != hipSuccess) return e;
+  const Fp8Gemm g{xq, xs, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
+  if (p.out_dt == DT_FP32) return launch_gemm<DT_FP32>(g, stream);
+  if (p.out_dt == DT_BF16) return launch_gemm<DT_BF16>(g, stream);
+  return launch_gemm<DT_FP16>(g, stream);
 }
 
 }  // namespace ed

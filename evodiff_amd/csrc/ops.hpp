@@ -19,9 +19,9 @@ hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, i
 hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride, int64_t N, int64_t K, uint8_t* q,
                                       uint8_t* scale, hipStream_t stream);
 
-// out[m][n] = bias[n] + sum_b 2^(xs[m][b] + ws[n / 128][b] - 254) sum_{k in block b} xq[m][k] * wq[n][k]
+// out[m][n] = bias[n] + sum_b 2^(xs[b][m] + ws[n / 128][b] - 254) sum_{k in block b} xq[m][k] * wq[n][k]
 struct Fp8Gemm {
-  const uint8_t *xq, *xs;  // (M, Kb * 128), (M, Kb)
+  const uint8_t *xq, *xs;  // (M, Kb * 128), (Kb, M)
   const uint8_t *wq, *ws;  // (N, Kb * 128), (ceil(N / 128), Kb)
   const float* bias;       // nullptr or [N]
   void* out;               // (M, N) of type out_dt
