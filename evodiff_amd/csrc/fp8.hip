@@ -67,25 +67,33 @@ __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
   return r;
 }
 
-// 16 lanes own a block of 128; the 16 blocks of a workgroup are the same channels of 16 rows.  TURNED: scales go to (kb, rows),
-// as the product reads them (16 rows' bytes side by side), instead of (rows, kb).
-template <int DT, bool TURNED>
+// 16 lanes own a block of 128; a workgroup takes U blocks of 16 rows, all loads first.  TURNED: scales go to (kb, rows), as the
+// product reads them (16 rows' bytes side by side), instead of (rows, kb).
+template <int DT, int U, bool TURNED>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, long row_stride, long rows, int kb, long K,
                                                             bool wide, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
-  const long row = blockIdx.x / kb * 16 + (threadIdx.x >> 4);
-  const int b = (int)(blockIdx.x % kb), l = threadIdx.x & 15;
+  const int chunks = (kb + U - 1) / U;
+  const long row = blockIdx.x / chunks * 16 + (threadIdx.x >> 4);
+  const int b0 = (int)(blockIdx.x % chunks) * U, l = threadIdx.x & 15;
   if (row >= rows) return;
-  float v[8];
-  load8<DT>((const typename Elem<DT>::T*)x + row * row_stride, (long)b * FP8_BLOCK + l * 8, K, wide, v);
-  unsigned a = amax8(v);
+  const typename Elem<DT>::T* src = (const typename Elem<DT>::T*)x + row * row_stride;
+  float v[U][8];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    const unsigned c = (unsigned)__shfl_xor((int)a, o);
-    a = c > a ? c : a;
+  for (int u = 0; u < U; ++u) load8<DT>(src, (long)(b0 + u) * FP8_BLOCK + l * 8, K, wide, v[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int b = b0 + u;
+    if (b >= kb) break;
+    unsigned a = amax8(v[u]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const unsigned c = (unsigned)__shfl_xor((int)a, o);
+      a = c > a ? c : a;
+    }
+    const int byte = scale_byte(a);
+    *(uint2*)(q + (row * kb + b) * FP8_BLOCK + l * 8) = pack8(v[u], inverse_scale(byte));
+    if (l == 0) scale[TURNED ? b * rows + row : row * kb + b] = (uint8_t)byte;
   }
-  const int byte = scale_byte(a);
-  *(uint2*)(q + (row * kb + b) * FP8_BLOCK + l * 8) = pack8(v, inverse_scale(byte));
-  if (l == 0) scale[TURNED ? b * rows + row : row * kb + b] = (uint8_t)byte;
 }
 
 // One workgroup per 128 x 128 weights: thread (r, c) holds columns 8c .. 8c + 7 of rows r, r + 16, ...
@@ -150,9 +158,18 @@ __device__ __forceinline__ float scale_of(int byte) {  // 2^(byte - 127)
   return byte == 0 ? __uint_as_float(0x400000u) : byte == 255 ? __builtin_nanf("") : __uint_as_float((unsigned)byte << 23);
 }
 
-__device__ __forceinline__ void copy16(const uint8_t* src, char* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// Memory -> LDS copies and the scale loads are buffer instructions: they are bounded by the buffer (bytes past it read as zero:
+// rows behind the last need no clamp), take the step of K as a scalar offset, and unlike global ones leave the waits
+// for LDS reads countable.
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_of(const uint8_t* p, long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(unsigned)(bytes < 0xfffffff0L ? bytes : 0xfffffff0L), 0x00020000);
+}
+__device__ __forceinline__ void copy16(buffer_t src, unsigned lane_off, unsigned off, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16, (int)lane_off, (int)off, 0, 0);
+}
+__device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsigned off) {
+  return __builtin_amdgcn_raw_buffer_load_b8(src, (int)lane_off, (int)off, 0);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -194,37 +211,32 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   const long m0 = (long)tile_m * BM, n0 = (long)tile_n * BN, pitch = (long)g.kb * FP8_BLOCK;
   const int T = g.kb;
 
-  // copies: lane -> (row of 8, physical chunk); rows past the end repeat the last one
+  // copies: lane -> (row of 8, physical chunk)
   const int chunk0 = ((lane & 7) ^ (lane >> 4)) * 16, chunk1 = ((lane & 7) ^ (4 + (lane >> 4))) * 16;
   unsigned off[NG];
 #pragma unroll
   for (int j = 0; j < GX; ++j) {
-    const int row = (wid * GX + j) * 8 + (lane >> 3), left = (int)(g.M - 1 - m0 < BM ? g.M - 1 - m0 : BM);
-    off[j] = (unsigned)((row < left ? row : left) * pitch) + ((wid * GX + j) & 1 ? chunk1 : chunk0);
+    const int row = (wid * GX + j) * 8 + (lane >> 3);
+    off[j] = (unsigned)(row * pitch) + ((wid * GX + j) & 1 ? chunk1 : chunk0);
   }
 #pragma unroll
   for (int j = 0; j < GW; ++j) {
-    const int lr = (wid * GW + j) * 8 + (lane >> 3), left = (int)(g.N - 1 - n0 < BN ? g.N - 1 - n0 : BN);
+    const int lr = (wid * GW + j) * 8 + (lane >> 3);
     const int ch = (lr & ~31) + 8 * ((lr & 15) >> 2) + 4 * ((lr >> 4) & 1) + (lr & 3);
-    off[GX + j] = (unsigned)((ch < left ? ch : left) * pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
+    off[GX + j] = (unsigned)(ch * pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
   }
-  const uint8_t* x_src = g.xq + m0 * pitch;
-  const uint8_t* w_src = g.wq + n0 * pitch;
-  auto copy = [&](int j, char* stage) {  // piece j of the step that x_src and w_src stand at
-    if (j < GX) copy16(x_src + off[j], stage + (wid * GX + j) * 1024);
-    else copy16(w_src + off[j], stage + BM * 128 + (wid * GW + j - GX) * 1024);
+  const buffer_t x_src = buffer_of(g.xq + m0 * pitch, (g.M - m0) * pitch);
+  const buffer_t w_src = buffer_of(g.wq + n0 * pitch, (g.N - n0) * pitch);
+  auto copy = [&](int j, unsigned at, char* stage) {  // piece j of the step at byte `at` of the rows
+    if (j < GX) copy16(x_src, off[j], at, stage + (wid * GX + j) * 1024);
+    else copy16(w_src, off[j], at, stage + BM * 128 + (wid * GW + j - GX) * 1024);
   };
 
   // scales: a lane's row in each of the WTM fragments; the wave's channels lie in one block of 128
-  unsigned sx_off[WTM];
-#pragma unroll
-  for (int i = 0; i < WTM; ++i) {
-    const long m = m0 + wr * 16 * WTM + i * 16 + fr;
-    sx_off[i] = (unsigned)(m < g.M ? m : g.M - 1);
-  }
+  const unsigned mw = (unsigned)(m0 + wr * 16 * WTM + fr);
   const long nw = n0 + wc * 16 * WTN;
-  const uint8_t* sw_src = g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb;
-  const uint8_t* sx_src = g.xs;  // (kb, M)
+  const buffer_t sx_src = buffer_of(g.xs, g.M * (long)T);  // (kb, M)
+  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb, T);
 
   const int swz = (fq ^ ((fr >> 1) & 7)) << 4;
   const int x_rd = (wr * 16 * WTM + fr) * 128, w_rd = BM * 128 + (wc * 16 * WTN + fr) * 128;
@@ -238,40 +250,34 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   i32x8 X[WTM], W[RING];
   int sx[WTM], sx_next[WTM], sw, sw_next;
 
-  // step t = 0 in flight, its first fragments, step 1's copies
+  // step 0, its first fragments, step 1's copies
 #pragma unroll
-  for (int j = 0; j < NG; ++j) copy(j, lds);
+  for (int j = 0; j < NG; ++j) copy(j, 0, lds);
 #pragma unroll
-  for (int i = 0; i < WTM; ++i) sx[i] = sx_src[sx_off[i]];
-  sw = sw_src[0];
+  for (int i = 0; i < WTM; ++i) sx[i] = load_byte(sx_src, mw + i * 16, 0);
+  sw = load_byte(sw_src, 0, 0);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < WTM; ++i) { put(X[i], 0, read(lds, x_rd + i * 2048, 0)); put(X[i], 1, read(lds, x_rd + i * 2048, 1)); }
 #pragma unroll
   for (int j = 0; j < 2; ++j) { put(W[j], 0, read(lds, w_rd + j * 2048, 0)); put(W[j], 1, read(lds, w_rd + j * 2048, 1)); }
   // The copies run two steps ahead; past the last step they repeat its block (in bounds, into a stage nobody reads).
-  int ahead = 0;
-  auto advance = [&]() {
-    const long d = ++ahead < T ? FP8_BLOCK : 0;
-    x_src += d;
-    w_src += d;
-  };
-  advance();
+  const unsigned last = (unsigned)(T - 1);
+  unsigned at = (last < 1 ? last : 1) * FP8_BLOCK;
 #pragma unroll
-  for (int j = 0; j < NG; ++j) copy(j, lds + STAGE);
+  for (int j = 0; j < NG; ++j) copy(j, at, lds + STAGE);
 
   for (int t = 0; t < T; ++t) {
     char* const here = lds + (t & 1) * STAGE;
     const char* const there = lds + (1 - (t & 1)) * STAGE;
-    const int more = t + 1 < T ? 1 : 0;
-    sx_src += more ? g.M : 0;
-    sw_src += more;
+    const unsigned next = (unsigned)t < last ? t + 1 : last;
+    const unsigned sx_at = next * (unsigned)g.M;
+    at = ((unsigned)t + 2 < last ? t + 2 : last) * FP8_BLOCK;
 #pragma unroll
     for (int j = 0; j < WTN; ++j) {
       if (j == JB) {
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();  // (drains this wave's copies and reads)
-        advance();
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -285,13 +291,13 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
             const int f = 2 + r / 2, want = f < RING ? r : (f - RING + 1) * WTM + (r & 1);
             if (want == slot) put(W[f % RING], r & 1, read(here, w_rd + f * 2048, r & 1));
           }
-          if (slot >= 4 && slot < 4 + WTM) sx_next[slot - 4] = sx_src[sx_off[slot - 4]];  // the next step's scales
-          if (slot == 4) sw_next = sw_src[0];
+          if (slot >= 4 && slot < 4 + WTM) sx_next[slot - 4] = load_byte(sx_src, mw + (slot - 4) * 16, sx_at);  // the next step's scales
+          if (slot == 4) sw_next = load_byte(sw_src, 0, next);
         } else {
           constexpr int COPY_SLOTS = (WTN - JB) * WTM;
           const int after = slot - JB * WTM;
 #pragma unroll
-          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, here);
+          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, at, here);
           // the next step's first two channel fragments: slot 0 is free, slot 1 too unless row JB of instructions reads it
           constexpr int W1_AT = JB % RING == 1 ? WTM : 2;
           if (after < 2) put(W[0], after, read(there, w_rd, after));
@@ -417,12 +423,23 @@ template <bool TURNED>
 static hipError_t quantize_rows(const void* x, int dt, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q, uint8_t* scale,
                                 hipStream_t stream) {
   const int kb = (int)fp8_blocks(K);
-  const dim3 grid((unsigned)((rows + 15) / 16 * kb));
   const bool wide = wide_rows(x, dt, row_stride);
-#define ED_GO(DT) hipLaunchKernelGGL((quantize_rows_kernel<DT, TURNED>), grid, dim3(256), 0, stream, x, (long)row_stride, (long)rows, kb, (long)K, wide, q, scale)
-  if (dt == DT_FP32) ED_GO(DT_FP32);
-  else if (dt == DT_BF16) ED_GO(DT_BF16);
-  else ED_GO(DT_FP16);
+  // four blocks a thread where that still leaves every CU eight workgroups, else one
+  const int64_t bands = (rows + 15) / 16;
+  const int u = bands * ((kb + 3) / 4) >= 2048 ? 4 : 1;
+  const dim3 grid((unsigned)(bands * ((kb + u - 1) / u)));
+#define ED_GO(DT)                                                                                                          \
+  if (u == 4) ED_GO_U(DT, 4);                                                                                              \
+  else ED_GO_U(DT, 1)
+#define ED_GO_U(DT, U) hipLaunchKernelGGL((quantize_rows_kernel<DT, U, TURNED>), grid, dim3(256), 0, stream, x, (long)row_stride, (long)rows, kb, (long)K, wide, q, scale)
+  if (dt == DT_FP32) {
+    ED_GO(DT_FP32);
+  } else if (dt == DT_BF16) {
+    ED_GO(DT_BF16);
+  } else {
+    ED_GO(DT_FP16);
+  }
+#undef ED_GO_U
 #undef ED_GO
   return hipGetLastError();
 }
