@@ -81,7 +81,7 @@ def load():
     lib.ed_probe_read.argtypes = [vp, C.POINTER(EdProbeStat), vp]
     lib.ed_fp8_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
     lib.ed_fp8_quantize_weight.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
-    lib.ed_fp8_linear_workspace.argtypes = [i64, i64, i64, i32]
+    lib.ed_fp8_linear_workspace.argtypes = [i64, i64, i64, i32, i32]
     lib.ed_fp8_linear_workspace.restype = i64
     lib.ed_fp8_linear.argtypes = [vp, i32, i64, vp, vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp]
     lib.ed_token_logprobs_workspace.argtypes = [i64, i64, i32]

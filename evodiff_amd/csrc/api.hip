@@ -1570,10 +1570,11 @@ bool plain_dtype(int dt) { return dt == ED_DT_FP32 || dt == ED_DT_BF16 || dt == 
 bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 constexpr int64_t MAX_DIM = 1LL << 30;     // rows, columns and classes each stay below this
 constexpr int64_t MAX_BLOCKS = 1LL << 28;  // 128-value blocks (or tiles) of one operand
+constexpr int64_t MAX_K = 1LL << 22;       // a tile's rows are addressed with 32 bits
 
 int check_values(const char* what, const void* p, int dt, int64_t row_stride, int64_t rows, int64_t K) {
   if (!plain_dtype(dt)) return fail(ED_EINVAL, "%s: dtype must be fp32, bf16 or fp16 (got %d)", what, dt);
-  if (rows < 0 || rows >= MAX_DIM || K < 1 || K >= MAX_DIM || fp8_blocks(K) * rows >= MAX_BLOCKS)
+  if (rows < 0 || rows >= MAX_DIM || K < 1 || K > MAX_K || fp8_blocks(K) * rows >= MAX_BLOCKS)
     return fail(ED_EINVAL, "%s: %lld x %lld values are out of range", what, (long long)rows, (long long)K);
   if (row_stride < 0) return fail(ED_EINVAL, "%s: negative row stride", what);
   if (rows > 0 && !p) return fail(ED_EINVAL, "%s: null pointer", what);
@@ -1617,9 +1618,9 @@ int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, i
   return ED_OK;
 }
 
-int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype) {
-  if (M < 1 || N < 1 || K < 1 || M >= MAX_DIM || N >= MAX_DIM || K >= MAX_DIM) return 0;
-  return fp8_linear_workspace(M, N, K, x_dtype == ED_DT_E4M3);
+int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype, int out_dtype) {
+  if (M < 1 || N < 1 || K < 1 || M >= MAX_DIM || N >= MAX_DIM || K > MAX_K) return 0;
+  return fp8_linear_workspace(M, N, K, x_dtype == ED_DT_E4M3, out_dtype == ED_DT_FP32);
 }
 
 int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
@@ -1627,7 +1628,7 @@ int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint
                   int64_t K, void* workspace_dev, int64_t workspace_bytes, void* stream) {
   const bool quantised = x_dtype == ED_DT_E4M3;
   if (quantised) {
-    if (M < 0 || M >= MAX_DIM || K < 1 || K >= MAX_DIM || fp8_blocks(K) * M >= MAX_BLOCKS)
+    if (M < 0 || M >= MAX_DIM || K < 1 || K > MAX_K || fp8_blocks(K) * M >= MAX_BLOCKS)
       return fail(ED_EINVAL, "x: %lld x %lld values are out of range", (long long)M, (long long)K);
     if (row_stride != fp8_blocks(K) * FP8_BLOCK) return fail(ED_EINVAL, "quantised rows are ceil(K / 128) * 128 bytes apart");
     if (misaligned(x_dev, 16)) return fail(ED_EINVAL, "quantised rows must be aligned to 16 bytes");
@@ -1642,7 +1643,7 @@ int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint
     return fail(ED_EINVAL, "null x/scale/weight/out pointer");
   if (misaligned(weight_dev, 16)) return fail(ED_EINVAL, "the weight must be aligned to 16 bytes");
   if (misaligned(out_dev, (size_t)dt_bytes(out_dtype)) || misaligned(bias_dev, 4)) return fail(ED_EINVAL, "out/bias: not aligned to their element");
-  const int64_t need = fp8_linear_workspace(M, N, K, quantised);
+  const int64_t need = fp8_linear_workspace(M, N, K, quantised, out_dtype == ED_DT_FP32);
   if (need > 0 && (!workspace_dev || workspace_bytes < need || misaligned(workspace_dev, 16)))
     return fail(ED_EINVAL, "workspace: %lld bytes at a 16-byte boundary are needed (ed_fp8_linear_workspace)", (long long)need);
   const Fp8Linear p{x_dev, x_dtype, row_stride, x_scale_dev, weight_dev, weight_scale_dev, bias_dev, out_dev, out_dtype,

@@ -9,6 +9,8 @@
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
+#include <cstdlib>
+#include <cstdio>
 
 namespace ed {
 namespace {
@@ -176,25 +178,30 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 // Tiled product.  Four waves, 2 (rows) x 2 (channels), own a tile of 32 WTM rows x 32 WTN channels, a wave 16 WTM x 16 WTN as
 // WTN x WTM instructions of 16 x 16 x 128: one per block of K and pair of fragments, its scales beside it.
 //
-// Step of K (one block): rows of 128 bytes of both operands, copied memory -> LDS a step ahead into one of two stages.  The
-// 16-byte chunk c of tile row r lies at chunk c ^ (r >> 1 & 7) (the copy's source addresses are permuted, its image is
+// Step of K (one block): rows of 128 bytes of both operands, copied memory -> LDS into a ring of S stages, S - 1 steps ahead.
+// The 16-byte chunk c of tile row r lies at chunk c ^ (r >> 1 & 7) (the copy's source addresses are permuted, its image is
 // lane-linear): the 16 rows of a fragment read then fall on 16 different slots of the banks.
 //
-// Order inside a step.  A wave's channel fragments pass through a ring of four, its row fragments stay for the step.  Once
-// the last channel fragment of the step is read (row of instructions JB), the one barrier of the step: behind it the next
-// stage has landed and this one is free.  The rows of instructions left cover the reads of the next step's first fragments and
-// the copies of the step after, so that neither the barrier nor a read leaves the matrix pipe without work.  The
-// order is pinned (sched_barrier): at most two auxiliary instructions behind each matrix instruction.
+// Order inside a step.  A wave's channel fragments pass through a ring of four, its row fragments stay for the step and are
+// replaced in place during the last row of instructions.  Once the last channel fragment of the step is read (row of
+// instructions JB), the one barrier of the step: behind it the next stage has landed (the copies of the steps after it
+// stay in flight: they are counted, not drained) and this one is free.  The rows of instructions left cover the reads
+// of the next step's first fragments and the copies into the free stage, so that neither the barrier nor a read leaves the
+// matrix pipe without work.  The order is pinned (sched_barrier): at most a few auxiliary instructions behind each matrix one.
+//
+// EXACT: the fragments are widened to bf16 (scales applied) and multiplied four times K = 32.
+// A cut K loop (gridDim.y > 1) stores its part of the sums, fp32 without bias, to out + blockIdx.y * M * N.
 //
 // The channels of an LDS tile are permuted within 32 so that two instructions give a lane eight consecutive ones: 16-byte stores.
 // ---------------------------------------------------------------------------------------------------
-template <int WTM, int WTN, int OUT_DT>
+template <int WTM, int WTN, int S, int OUT_DT, bool EXACT>
 __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
   constexpr int BM = 32 * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
   constexpr int GX = BM / 32, GW = BN / 32, NG = GX + GW;  // 8-row copies a wave makes of each operand
-  constexpr int RING = 4, JB = WTN > 4 ? WTN - 3 : WTN - 2;  // the barrier stands before row JB of instructions
+  constexpr int RING = 4, JB = WTN > 4 ? WTN - 3 : WTN > 2 ? WTN - 2 : 1;  // the barrier stands before row JB of instructions
   static_assert(JB >= WTN - RING + 1 && JB >= 1, "every channel fragment of a step is read in front of its barrier");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  static_assert((S & (S - 1)) == 0 && S >= 2, "the ring index is masked");
+  __shared__ __attribute__((aligned(1024))) char lds[S * STAGE];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4, wr = wid >> 1, wc = wid & 1;
 
@@ -209,7 +216,8 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     tile_m = 4 * band + in - tile_n * high;
   }
   const long m0 = (long)tile_m * BM, n0 = (long)tile_n * BN, pitch = (long)g.kb * FP8_BLOCK;
-  const int T = g.kb;
+  // blocks of K of this workgroup (never none: the launcher cuts into no more pieces than there are)
+  const int first = (int)((long)g.kb * blockIdx.y / gridDim.y), T = (int)((long)g.kb * (blockIdx.y + 1) / gridDim.y) - first;
 
   // copies: lane -> (row of 8, physical chunk)
   const int chunk0 = ((lane & 7) ^ (lane >> 4)) * 16, chunk1 = ((lane & 7) ^ (4 + (lane >> 4))) * 16;
@@ -227,7 +235,10 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   }
   const buffer_t x_src = buffer_of(g.xq + m0 * pitch, (g.M - m0) * pitch);
   const buffer_t w_src = buffer_of(g.wq + n0 * pitch, (g.N - n0) * pitch);
-  auto copy = [&](int j, unsigned at, char* stage) {  // piece j of the step at byte `at` of the rows
+  // Past the last step the copies repeat its block (in bounds, into a stage nobody reads).
+  const int last = T - 1;
+  auto copy = [&](int j, int t, char* stage) {  // piece j of step t
+    const unsigned at = (unsigned)(first + (t < last ? t : last)) * FP8_BLOCK;
     if (j < GX) copy16(x_src, off[j], at, stage + (wid * GX + j) * 1024);
     else copy16(w_src, off[j], at, stage + BM * 128 + (wid * GW + j - GX) * 1024);
   };
@@ -235,8 +246,8 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   // scales: a lane's row in each of the WTM fragments; the wave's channels lie in one block of 128
   const unsigned mw = (unsigned)(m0 + wr * 16 * WTM + fr);
   const long nw = n0 + wc * 16 * WTN;
-  const buffer_t sx_src = buffer_of(g.xs, g.M * (long)T);  // (kb, M)
-  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb, T);
+  const buffer_t sx_src = buffer_of(g.xs, g.M * (long)g.kb);  // (kb, M)
+  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb, g.kb);
 
   const int swz = (fq ^ ((fr >> 1) & 7)) << 4;
   const int x_rd = (wr * 16 * WTM + fr) * 128, w_rd = BM * 128 + (wc * 16 * WTN + fr) * 128;
@@ -248,56 +259,70 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
 
   f32x4 acc[WTN][WTM] = {};
   i32x8 X[WTM], W[RING];
+  bf16x8 XW[EXACT ? WTM : 1][4], WW[4];
   int sx[WTM], sx_next[WTM], sw, sw_next;
 
-  // step 0, its first fragments, step 1's copies
+  // step 0 and its first fragments, copies of the S - 1 steps behind it
 #pragma unroll
   for (int j = 0; j < NG; ++j) copy(j, 0, lds);
 #pragma unroll
-  for (int i = 0; i < WTM; ++i) sx[i] = load_byte(sx_src, mw + i * 16, 0);
-  sw = load_byte(sw_src, 0, 0);
-  __syncthreads();
+  for (int i = 0; i < WTM; ++i) sx[i] = load_byte(sx_src, mw + i * 16, (unsigned)first * (unsigned)g.M);
+  sw = load_byte(sw_src, 0, (unsigned)first);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int k = 1; k < S; ++k)
+#pragma unroll
+    for (int j = 0; j < NG; ++j) copy(j, k, lds + k * STAGE);
 #pragma unroll
   for (int i = 0; i < WTM; ++i) { put(X[i], 0, read(lds, x_rd + i * 2048, 0)); put(X[i], 1, read(lds, x_rd + i * 2048, 1)); }
 #pragma unroll
   for (int j = 0; j < 2; ++j) { put(W[j], 0, read(lds, w_rd + j * 2048, 0)); put(W[j], 1, read(lds, w_rd + j * 2048, 1)); }
-  // The copies run two steps ahead; past the last step they repeat its block (in bounds, into a stage nobody reads).
-  const unsigned last = (unsigned)(T - 1);
-  unsigned at = (last < 1 ? last : 1) * FP8_BLOCK;
-#pragma unroll
-  for (int j = 0; j < NG; ++j) copy(j, at, lds + STAGE);
 
   for (int t = 0; t < T; ++t) {
-    char* const here = lds + (t & 1) * STAGE;
-    const char* const there = lds + (1 - (t & 1)) * STAGE;
-    const unsigned next = (unsigned)t < last ? t + 1 : last;
-    const unsigned sx_at = next * (unsigned)g.M;
-    at = ((unsigned)t + 2 < last ? t + 2 : last) * FP8_BLOCK;
+    char* const here = lds + (t & (S - 1)) * STAGE;
+    const char* const there = lds + ((t + 1) & (S - 1)) * STAGE;
+    const unsigned next = (unsigned)(first + (t < last ? t + 1 : last)), sx_at = next * (unsigned)g.M;
 #pragma unroll
     for (int j = 0; j < WTN; ++j) {
       if (j == JB) {
+        // Behind the copies of step t + 1 at least those of S - 2 steps and this step's scale loads were issued: with no more
+        // than that many outstanding they have landed.  This wave's reads of the stage are in registers.
         __builtin_amdgcn_sched_barrier(0);
-        __syncthreads();  // (drains this wave's copies and reads)
+        constexpr int OUT = (S - 2) * NG + WTM + 1;
+        static_assert(OUT < 64, "the counter has six bits");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < WTM; ++i) {
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, sw, 0, sx[i]);
+        if constexpr (EXACT) {
+          if (i == 0)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) WW[h] = widen(W[j % RING], h, scale_of(sw));
+          if (j == 0)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) XW[i][h] = widen(X[i], h, scale_of(sx[i]));
+#pragma unroll
+          for (int h = 0; h < 4; ++h) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(WW[h], XW[i][h], acc[j][i], 0, 0, 0);
+        } else {
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, sw, 0, sx[i]);
+        }
         const int slot = j * WTM + i;
         if (j < JB) {
           // channel fragments 2 .. WTN - 1, two reads each, as soon as their slot of the ring is free
 #pragma unroll
           for (int r = 0; r < 2 * (WTN - 2); ++r) {
-            const int f = 2 + r / 2, want = f < RING ? r : (f - RING + 1) * WTM + (r & 1);
+            const int f = 2 + r / 2, want = f < RING ? (r < JB * WTM ? r : JB * WTM - 1) : (f - RING + 1) * WTM + (r & 1);
             if (want == slot) put(W[f % RING], r & 1, read(here, w_rd + f * 2048, r & 1));
           }
-          if (slot >= 4 && slot < 4 + WTM) sx_next[slot - 4] = load_byte(sx_src, mw + (slot - 4) * 16, sx_at);  // the next step's scales
-          if (slot == 4) sw_next = load_byte(sw_src, 0, next);
+          constexpr int AT = JB * WTM >= 4 + WTM ? 4 : 0;  // the next step's scales
+          if (slot >= AT && slot < AT + WTM) sx_next[slot - AT] = load_byte(sx_src, mw + (slot - AT) * 16, sx_at);
+          if (slot == AT) sw_next = load_byte(sw_src, 0, next);
         } else {
           constexpr int COPY_SLOTS = (WTN - JB) * WTM;
           const int after = slot - JB * WTM;
 #pragma unroll
-          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, at, here);
+          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, t + S, here);
           // the next step's first two channel fragments: slot 0 is free, slot 1 too unless row JB of instructions reads it
           constexpr int W1_AT = JB % RING == 1 ? WTM : 2;
           if (after < 2) put(W[0], after, read(there, w_rd, after));
@@ -306,6 +331,10 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
             put(X[i], 0, read(there, x_rd + i * 2048, 0));  // in place: X[i] has done its last instruction of the step
             put(X[i], 1, read(there, x_rd + i * 2048, 1));
             sx[i] = sx_next[i];
+            if (W1_AT >= COPY_SLOTS && i == WTM - 1) {
+              put(W[1], 0, read(there, w_rd + 2048, 0));
+              put(W[1], 1, read(there, w_rd + 2048, 1));
+            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -313,94 +342,67 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     }
     sw = sw_next;
   }
-  __syncthreads();  // (no copy may land once this workgroup's shared memory is another's)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no copy may land once this workgroup's shared memory is another's)
 
   // ---- results: acc[2 J][i], acc[2 J + 1][i] are channels nw + 32 J + 8 fq + 0 .. 3, 4 .. 7 of row i * 16 + fr
   typedef typename Elem<OUT_DT>::T T_out;
   typedef __attribute__((ext_vector_type(8))) T_out V8;
-  T_out* const out = (T_out*)g.out;
+  T_out* const out = (T_out*)g.out + (gridDim.y > 1 ? (long)blockIdx.y * g.M * g.N : 0);
   const bool wide = (g.N & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const buffer_t bias = buffer_of((const uint8_t*)g.bias, g.bias ? g.N * 4 : 0);  // (reads as zero behind its end)
+  f32x4 b[WTN];
 #pragma unroll
-  for (int J = 0; J < WTN / 2; ++J) {
-    const long n = nw + 32 * J + 8 * fq;
-    float b[8];
+  for (int j = 0; j < WTN; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = g.bias && n + e < g.N ? g.bias[n + e] : 0.f;
+    for (int e = 0; e < 4; ++e)
+      b[j][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bias, (int)((nw + 32 * (j >> 1) + 8 * fq + 4 * (j & 1) + e) * 4), 0, 0));
 #pragma unroll
-    for (int i = 0; i < WTM; ++i) {
-      const long m = m0 + wr * 16 * WTM + i * 16 + fr;
-      if (m >= g.M) continue;
+  for (int i = 0; i < WTM; ++i) {
+    const long m = m0 + wr * 16 * WTM + i * 16 + fr;
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int J = 0; J < WTN / 2; ++J) {
+      const long n = nw + 32 * J + 8 * fq;
       T_out* const to = out + m * g.N + n;
       if (wide && n + 8 <= g.N) {
         V8 v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[e]);
+        for (int e = 0; e < 8; ++e) v[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[2 * J + (e >> 2)][e & 3]);
         *(V8*)to = v;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (n + e < g.N) to[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[e]);
+          if (n + e < g.N) to[e] = (T_out)(acc[2 * J + (e >> 2)][i][e & 3] + b[2 * J + (e >> 2)][e & 3]);
       }
     }
   }
 }
 
-// Any shape, operands straight from memory, a wave per 32 x 32 results; row scales as in the tiled kernel.
-__device__ __forceinline__ i32x8 load_fragment(const uint8_t* row, int fq) {
-  const i32x4 a = *(const i32x4*)(row + fq * 16), b = *(const i32x4*)(row + 64 + fq * 16);
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// out = bias + the parts of a cut K loop, added in order; eight values a thread
 template <int OUT_DT>
-__device__ __forceinline__ void store_out(void* out, long at, float v) {
-  ((typename Elem<OUT_DT>::T*)out)[at] = (typename Elem<OUT_DT>::T)v;
-}
-template <int OUT_DT>
-__global__ __launch_bounds__(256) void gemm_kernel(Fp8Gemm g) {
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int fr = lane & 15, fq = lane >> 4;
-  const long tiles_n = (g.N + 63) / 64;
-  const long m0 = blockIdx.x / tiles_n * 64 + (wid >> 1) * 32, n0 = blockIdx.x % tiles_n * 64 + (wid & 1) * 32;
-  const long pitch = (long)g.kb * FP8_BLOCK;
-  long rm[2], rn[2];
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int parts, const float* __restrict__ bias,
+                                                   void* __restrict__ out, long M, long N) {
+  typedef typename Elem<OUT_DT>::T T_out;
+  const long count = M * N;
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (long)gridDim.x * 1024) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i + 4 <= count && (count & 3) == 0) {
+#pragma unroll 4
+      for (int z = 0; z < parts; ++z) {
+        const f32x4 p = *(const f32x4*)(part + z * count + i);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    rm[i] = m0 + i * 16 + fr < g.M ? m0 + i * 16 + fr : g.M - 1;
-    rn[i] = n0 + i * 16 + fr < g.N ? n0 + i * 16 + fr : g.N - 1;
-  }
-  f32x4 acc[2][2] = {};
-  for (int b = 0; b < g.kb; ++b) {
-    i32x8 w[2], x[2];
-    int sw[2], sx[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      w[i] = load_fragment(g.wq + rn[i] * pitch + (long)b * FP8_BLOCK, fq);
-      x[i] = load_fragment(g.xq + rm[i] * pitch + (long)b * FP8_BLOCK, fq);
-      sw[i] = g.ws[(rn[i] >> 7) * g.kb + b];
-      sx[i] = g.xs[b * g.M + rm[i]];
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if constexpr (OUT_DT != DT_FP32) {
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[j], acc[i][j], 0, 0, 0, sw[i], 0, sx[j]);
-        } else {
-#pragma unroll
-          for (int s2 = 0; s2 < 4; ++s2)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(w[i], s2, scale_of(sw[i])), widen(x[j], s2, scale_of(sx[j])), acc[i][j], 0, 0, 0);
-        }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long m = m0 + j * 16 + fr;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const long n = n0 + i * 16 + fq * 4 + e;
-        if (m < g.M && n < g.N) store_out<OUT_DT>(g.out, m * g.N + n, acc[i][j][e] + (g.bias ? g.bias[n] : 0.f));
+        for (int e = 0; e < 4; ++e) v[e] += p[e];
       }
+    } else {
+      for (int z = 0; z < parts; ++z)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < count) v[e] += part[z * count + i + e];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < count) ((T_out*)out)[i + e] = (T_out)(v[e] + (bias ? bias[(i + e) % N] : 0.f));
+  }
 }
 
 // scale (rows, kb) -> (kb, rows)
@@ -461,28 +463,64 @@ hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride,
   return hipGetLastError();
 }
 
-template <int WTM, int WTN, int OUT_DT>
-static hipError_t launch_tile(const Fp8Gemm& g, hipStream_t stream) {
+// How a product is cut: the tile (in units of 32 rows and channels), and the pieces of its K loop.
+struct Plan {
+  int wtm, wtn, parts;
+};
+static Plan plan_of(int64_t M, int64_t N, int kb, bool exact) {
+  static const char* force = getenv("FT");
+  if (force) {
+    int a, b, c;
+    sscanf(force, "%d,%d,%d", &a, &b, &c);
+    return Plan{a, b, c < kb ? c : kb};
+  }
+  const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+  if (big >= 200 && !exact) return Plan{8, 8, 1};
+  if (M > 64) return Plan{4, 4, 1};
+  return Plan{2, 2, 1};
+}
+
+template <int WTM, int WTN, int S, int OUT_DT, bool EXACT>
+static hipError_t launch_tile(const Fp8Gemm& g, int parts, hipStream_t stream) {
   const int tiles_m = (int)((g.M + 32 * WTM - 1) / (32 * WTM)), tiles_n = (int)((g.N + 32 * WTN - 1) / (32 * WTN));
-  hipLaunchKernelGGL((tile_kernel<WTM, WTN, OUT_DT>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0, stream, g, tiles_m, tiles_n);
+  hipLaunchKernelGGL((tile_kernel<WTM, WTN, S, OUT_DT, EXACT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), 0, stream, g,
+                     tiles_m, tiles_n);
   return hipGetLastError();
+}
+
+template <int OUT_DT, bool EXACT>
+static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t stream) {
+  if constexpr (!EXACT) {
+    if (p.wtm == 8) return launch_tile<8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
+  }
+  if (p.wtm == 4) return launch_tile<4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
+  return launch_tile<2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
 }
 
 template <int OUT_DT>
-static hipError_t launch_gemm(const Fp8Gemm& g, hipStream_t stream) {
-  if constexpr (OUT_DT != DT_FP32) {
-    const int64_t big = ((g.M + 255) / 256) * ((g.N + 255) / 256);
-    if (big >= 200) return launch_tile<8, 8, OUT_DT>(g, stream);
-    if (g.M > 64) return launch_tile<4, 4, OUT_DT>(g, stream);
-  }
-  const dim3 grid((unsigned)(((g.N + 63) / 64) * ((g.M + 63) / 64)));
-  hipLaunchKernelGGL((gemm_kernel<OUT_DT>), grid, dim3(256), 0, stream, g);
+static hipError_t launch_gemm(const Fp8Gemm& g, void* partial, hipStream_t stream) {
+  constexpr bool EXACT = OUT_DT == DT_FP32;
+  const Plan p = plan_of(g.M, g.N, g.kb, EXACT);
+  if (p.parts == 1) return launch_plan<OUT_DT, EXACT>(g, p, stream);
+  Fp8Gemm part = g;
+  part.out = partial;
+  part.bias = nullptr;
+  const hipError_t e = launch_plan<DT_FP32, EXACT>(part, p, stream);
+  if (e != hipSuccess) return e;
+  const long blocks = (g.M * g.N + 1023) / 1024;
+  hipLaunchKernelGGL((join_kernel<OUT_DT>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, (const float*)partial,
+                     p.parts, g.bias, g.out, (long)g.M, (long)g.N);
   return hipGetLastError();
 }
 
-// workspace: the quantised rows (a multiple of 128 bytes), then their scales, (kb, rows)
-int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised) {
-  return M * fp8_blocks(K) * (quantised ? 1 : FP8_BLOCK + 1);
+// workspace: the quantised rows (a multiple of 128 bytes), their scales, (kb, rows), up to 16 bytes, then the parts of a cut K loop
+static int64_t scales_end(int64_t M, int64_t kb, bool quantised) {
+  return (M * kb * (quantised ? 1 : FP8_BLOCK + 1) + 15) / 16 * 16;
+}
+int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact) {
+  const int64_t kb = fp8_blocks(K);
+  const Plan p = plan_of(M, N, (int)kb, exact);
+  return scales_end(M, kb, quantised) + (p.parts > 1 ? p.parts * M * N * 4 : 0);
 }
 
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
@@ -502,9 +540,10 @@ hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   }
   if (e != hipSuccess) return e;
   const Fp8Gemm g{xq, xs, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
-  if (p.out_dt == DT_FP32) return launch_gemm<DT_FP32>(g, stream);
-  if (p.out_dt == DT_BF16) return launch_gemm<DT_BF16>(g, stream);
-  return launch_gemm<DT_FP16>(g, stream);
+  void* const partial = (char*)p.workspace + scales_end(p.M, kb, p.x_dt == DT_E4M3);
+  if (p.out_dt == DT_FP32) return launch_gemm<DT_FP32>(g, partial, stream);
+  if (p.out_dt == DT_BF16) return launch_gemm<DT_BF16>(g, partial, stream);
+  return launch_gemm<DT_FP16>(g, partial, stream);
 }
 
 }  // namespace ed

@@ -198,7 +198,7 @@ at::Tensor linear_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& x_sc
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = N;
   at::Tensor out = at::empty(shape, x.options().dtype(ot));
-  const int64_t need = ed_fp8_linear_workspace(M, N, K, dt);
+  const int64_t need = ed_fp8_linear_workspace(M, N, K, dt, dtype_of(out, "out"));
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, x.options().dtype(at::kByte));
   check(ed_fp8_linear(r.data_ptr(), dt, r.stride(0), ptr_or_null<uint8_t>(x_scale), (const uint8_t*)weight.data_ptr(),

@@ -284,9 +284,9 @@ int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, i
  * x_dtype ED_DT_E4M3: x_dev and x_scale_dev are rows in the form above (row_stride = Kb * 128).  Any other x_dtype: x_dev holds
  * plain values, which are brought to that form first (x_scale_dev is ignored) - the result is the same, bit for bit, as
  * of ed_fp8_quantize_rows and a product on its outputs.  bias_dev: fp32 [N] or NULL.
- * workspace_dev: at least ed_fp8_linear_workspace(M, N, K, x_dtype) bytes, 16-byte aligned (NULL where that is 0); its contents
+ * workspace_dev: at least ed_fp8_linear_workspace(M, N, K, x_dtype, out_dtype) bytes, 16-byte aligned (NULL where that is 0); its contents
  * do not matter before or after the call. */
-int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype);
+int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype, int out_dtype);
 int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
                   const uint8_t* weight_scale_dev, const float* bias_dev, void* out_dev, int out_dtype, int64_t M, int64_t N,
                   int64_t K, void* workspace_dev, int64_t workspace_bytes, void* stream);

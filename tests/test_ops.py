@@ -137,7 +137,7 @@ def test_refusals_of_the_c_entry_points():
     refused(linear(n=0), "range")
     refused(linear(k=0), "range")
     refused(linear(m=1 << 29, n=1 << 20, k=1), "range")
-    need = lib.ed_fp8_linear_workspace(4096, 8, 256, 1)
+    need = lib.ed_fp8_linear_workspace(4096, 8, 256, 1, 1)
     assert need >= 4096 * 2 * 129
     refused(linear(m=4096, wb=need - 1), "workspace")
     refused(linear(m=4096, wk=None, wb=need), "workspace")
@@ -305,9 +305,9 @@ def test_linear_types_layouts_and_edges(dev, m, out_dtype):
     lib, x = _lib.load(), base[:, 0, :k].contiguous()
     guard = torch.full((m * n + 64,), 7.0, dtype=out_dtype, device=dev)
     out = guard[32:32 + m * n]
-    need = lib.ed_fp8_linear_workspace(m, n, k, _lib.DT_FP16)
-    ws = torch.empty(need + 16, dtype=torch.uint8, device=dev)
     code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[out_dtype]
+    need = lib.ed_fp8_linear_workspace(m, n, k, _lib.DT_FP16, code)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device=dev)
     _lib.check(lib.ed_fp8_linear(x.data_ptr(), _lib.DT_FP16, k, None, weight.q.data_ptr(), weight.scale.data_ptr(), None,
                                  out.data_ptr(), code, m, n, k, ws.data_ptr() if need else None, need,
                                  torch.cuda.current_stream().cuda_stream))
