@@ -378,6 +378,148 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   }
 }
 
+// ---------------------------------------------------------------------------------------------------
+// Few rows (up to 16 MT): the weights are streamed once and bound the time, so one launch does it all.  A workgroup owns
+// 16 NT channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as
+// fragments straight from memory, the next block's in flight, and brings the rows to 8 bits in registers - the four lanes that
+// hold a row's block find its largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
+// ---------------------------------------------------------------------------------------------------
+// 32 values of a row: columns k0 .. k0 + 15 and k0 + 64 .. k0 + 79, zeros behind K
+template <int DT>
+struct RowPart {
+  float v[4][8];
+  __device__ __forceinline__ void load(const void* x, long row_at, long k0, long K, bool on, bool wide) {
+    typedef typename Elem<DT>::T T;
+    const T* row = (const T*)x + row_at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (on) load8<DT>(row, k0 + (i >> 1) * 64 + (i & 1) * 8, K, wide, v[i]);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ int quantise(i32x8& f) {  // -> scale byte
+    unsigned a = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned c = amax8(v[i]);
+      a = c > a ? c : a;
+    }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+      const unsigned c = (unsigned)__shfl_xor((int)a, o);
+      a = c > a ? c : a;
+    }
+    const int byte = scale_byte(a);
+    const float inv = inverse_scale(byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint2 p = pack8(v[i], inv);
+      f[2 * i] = (int)p.x;
+      f[2 * i + 1] = (int)p.y;
+    }
+    return byte;
+  }
+};
+
+struct FewRows {
+  const void* x;
+  long row_stride, K;
+  const uint8_t* x_scale;  // x in 8 bits only: (M, kb)
+  bool wide;
+};
+
+template <int DT, bool EXACT, int MT, int NT>
+__global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  f32x4* const sums = (f32x4*)smem;  // [wave][NT][MT][64]
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
+  const int fr = lane & 15, fq = lane >> 4;
+  const long n0 = (long)blockIdx.x * 16 * NT, pitch = (long)g.kb * FP8_BLOCK;
+  const uint8_t* w_row[NT];
+  const uint8_t* ws_row[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const long n = n0 + j * 16 + fr < g.N ? n0 + j * 16 + fr : g.N - 1;  // (channels past the end repeat the last, unstored)
+    w_row[j] = g.wq + n * pitch + fq * 16;
+    ws_row[j] = g.ws + (n >> 7) * g.kb;
+  }
+  f32x4 acc[NT][MT] = {};
+  i32x4 w_next[NT][2];
+  int sw_next[NT];
+  auto fetch = [&](int b) {
+    if (b >= g.kb) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      w_next[j][0] = *(const i32x4*)(w_row[j] + (long)b * FP8_BLOCK);
+      w_next[j][1] = *(const i32x4*)(w_row[j] + (long)b * FP8_BLOCK + 64);
+      sw_next[j] = ws_row[j][b];
+    }
+  };
+  fetch(wid);
+  for (int b = wid; b < g.kb; b += waves) {
+    i32x8 W[NT], X[MT];
+    int sw[NT], sx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const long m = i * 16 + fr;
+      const bool on = m < g.M;
+      if constexpr (DT == DT_E4M3) {
+        const uint8_t* q = (const uint8_t*)r.x + (on ? m : 0) * pitch + (long)b * FP8_BLOCK + fq * 16;
+        X[i] = __builtin_shufflevector(*(const i32x4*)q, *(const i32x4*)(q + 64), 0, 1, 2, 3, 4, 5, 6, 7);
+        sx[i] = r.x_scale[(on ? m : 0) * g.kb + b];
+      } else {
+        RowPart<DT> part;
+        part.load(r.x, (on ? m : 0) * r.row_stride, (long)b * FP8_BLOCK + fq * 16, r.K, on, r.wide);
+        sx[i] = part.quantise(X[i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      W[j] = __builtin_shufflevector(w_next[j][0], w_next[j][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      sw[j] = sw_next[j];
+    }
+    fetch(b + waves);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if constexpr (EXACT) {
+        bf16x8 ww[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) ww[h] = widen(W[j], h, scale_of(sw[j]));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[h], widen(X[i], h, scale_of(sx[i])), acc[j][i], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j], X[i], acc[j][i], 0, 0, 0, sw[j], 0, sx[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[((wid * NT + j) * MT + i) * 64 + lane] = acc[j][i];
+  __syncthreads();
+  for (int at = tid; at < NT * MT * 64; at += (int)blockDim.x) {
+    f32x4 v = sums[at];
+    for (int w = 1; w < waves; ++w) v += sums[w * NT * MT * 64 + at];
+    const int l = at & 63, i = (at >> 6) % MT, j = (at >> 6) / MT;
+    const long m = i * 16 + (l & 15), n = n0 + j * 16 + (l >> 4) * 4;
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (n + e >= g.N) break;
+      const float y = v[e] + (g.bias ? g.bias[n + e] : 0.f);
+      const long o = m * g.N + n + e;
+      if constexpr (EXACT) ((float*)g.out)[o] = y;
+      else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)y;
+      else ((_Float16*)g.out)[o] = (_Float16)y;
+    }
+  }
+}
+
 // out = bias + the parts of a cut K loop, added in order; eight values a thread
 template <int OUT_DT>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int parts, const float* __restrict__ bias,
@@ -493,8 +635,30 @@ static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t strea
   if constexpr (!EXACT) {
     if (p.wtm == 8) return launch_tile<8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
   }
+  if (p.wtm == 5) return launch_tile<4, 4, 4, OUT_DT, EXACT>(g, p.parts, stream);
   if (p.wtm == 4) return launch_tile<4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
   return launch_tile<2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
+}
+
+constexpr int FEW_ROWS = 32;
+
+template <int DT, bool EXACT, int MT>
+static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
+  // Waves share K: up to 16, none without a block.  Two channel fragments a wave where that still gives every CU a workgroup (the
+  // rows are brought to 8 bits once for them), else one.
+  const int waves = g.kb < 16 ? g.kb : 16;
+  const bool two = (g.N + 31) / 32 >= 256;
+  const int nt = two ? 2 : 1;
+  const dim3 grid((unsigned)((g.N + 16 * nt - 1) / (16 * nt)));
+  const size_t smem = (size_t)waves * nt * MT * 1024;
+  if (two) hipLaunchKernelGGL((few_rows_kernel<DT, EXACT, MT, 2>), grid, dim3(64 * waves), smem, stream, g, r);
+  else hipLaunchKernelGGL((few_rows_kernel<DT, EXACT, MT, 1>), grid, dim3(64 * waves), smem, stream, g, r);
+  return hipGetLastError();
+}
+template <int DT>
+static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
+  if (g.out_dt == DT_FP32) return g.M <= 16 ? launch_few_rows<DT, true, 1>(g, r, stream) : launch_few_rows<DT, true, 2>(g, r, stream);
+  return g.M <= 16 ? launch_few_rows<DT, false, 1>(g, r, stream) : launch_few_rows<DT, false, 2>(g, r, stream);
 }
 
 template <int OUT_DT>
@@ -518,6 +682,7 @@ static int64_t scales_end(int64_t M, int64_t kb, bool quantised) {
   return (M * kb * (quantised ? 1 : FP8_BLOCK + 1) + 15) / 16 * 16;
 }
 int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact) {
+  if (M <= FEW_ROWS) return 0;
   const int64_t kb = fp8_blocks(K);
   const Plan p = plan_of(M, N, (int)kb, exact);
   return scales_end(M, kb, quantised) + (p.parts > 1 ? p.parts * M * N * 4 : 0);
@@ -525,6 +690,14 @@ int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bo
 
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   const int kb = (int)fp8_blocks(p.K);
+  if (p.M <= FEW_ROWS) {
+    const Fp8Gemm g{nullptr, nullptr, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
+    const FewRows r{p.x, (long)p.row_stride, (long)p.K, p.x_scale, p.x_dt != DT_E4M3 && wide_rows(p.x, p.x_dt, p.row_stride)};
+    if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, stream);
+    if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, stream);
+    if (p.x_dt == DT_FP16) return launch_few_rows<DT_FP16>(g, r, stream);
+    return launch_few_rows<DT_E4M3>(g, r, stream);
+  }
   const uint8_t* xq = (const uint8_t*)p.x;
   uint8_t* xs = (uint8_t*)p.workspace;
   hipError_t e;
