@@ -8,9 +8,8 @@
 
 #include <hip/hip_fp16.h>
 
-#include <type_traits>
-#include <cstdlib>
-#include <cstdio>
+#include <algorithm>
+#include <cmath>
 
 namespace ed {
 namespace {
@@ -143,21 +142,26 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
 // (2e-4), which those outputs are rounded by anyway.  fp32 outputs take the exact form: e4m3 values are exact in bf16, so are
 // their products in fp32, and the bf16 instruction keeps fp32 sums; it has half the rate.
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
-// values 8 s2 .. 8 s2 + 7 of a fragment times 2^(byte - 127) as bf16 (exact; magnitudes under 2^-126 vanish)
-__device__ __forceinline__ bf16x8 widen(const i32x8& v, int s2, float scale) {
-  bf16x8 r;
+// values 8 s2 .. 8 s2 + 7 of a fragment as bf16 (exact: the upper halves of their fp32 forms; a NaN stays one).  Four full-rate
+// instructions for four values; the scaled conversion straight to bf16 takes over three times as long.
+__device__ __forceinline__ bf16x8 widen(const i32x8& v, int s2) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  i32x4 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * s2 + i], scale, false);
-    const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * s2 + i], scale, true);
-    r[4 * i] = lo[0]; r[4 * i + 1] = lo[1]; r[4 * i + 2] = hi[0]; r[4 * i + 3] = hi[1];
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[2 * s2 + i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[2 * s2 + i], true);
+    r[2 * i] = (int)__builtin_amdgcn_perm(__float_as_uint(lo.y), __float_as_uint(lo.x), 0x07060302u);
+    r[2 * i + 1] = (int)__builtin_amdgcn_perm(__float_as_uint(hi.y), __float_as_uint(hi.x), 0x07060302u);
   }
-  return r;
+  return __builtin_bit_cast(bf16x8, r);
 }
-__device__ __forceinline__ float scale_of(int byte) {  // 2^(byte - 127)
-  return byte == 0 ? __uint_as_float(0x400000u) : byte == 255 ? __builtin_nanf("") : __uint_as_float((unsigned)byte << 23);
+// acc += part * 2^(sx + sw - 254) (a byte of 255 is a NaN)
+__device__ __forceinline__ void add_scaled(f32x4& acc, const f32x4& part, int sx, int sw) {
+  const int e = sx + sw - 254;
+  const bool bad = sx == 255 || sw == 255;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += bad ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(part[i], e);
 }
 
 // Memory -> LDS copies and the scale loads are buffer instructions: they are bounded by the buffer (bytes past it read as zero:
@@ -189,7 +193,7 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 // of the next step's first fragments and the copies into the free stage, so that neither the barrier nor a read leaves the
 // matrix pipe without work.  The order is pinned (sched_barrier): at most a few auxiliary instructions behind each matrix one.
 //
-// EXACT: the fragments are widened to bf16 (scales applied) and multiplied four times K = 32.
+// EXACT: the fragments are widened to bf16 and multiplied four times K = 32; a block's sums are scaled as they are added.
 // A cut K loop (gridDim.y > 1) stores its part of the sums, fp32 without bias, to out + blockIdx.y * M * N.
 //
 // The channels of an LDS tile are permuted within 32 so that two instructions give a lane eight consecutive ones: 16-byte stores.
@@ -260,6 +264,8 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   f32x4 acc[WTN][WTM] = {};
   i32x8 X[WTM], W[RING];
   bf16x8 XW[EXACT ? WTM : 1][4], WW[4];
+  f32x4 part[2];
+  int sx_now[WTM];
   int sx[WTM], sx_next[WTM], sw, sw_next;
 
   // step 0 and its first fragments, copies of the S - 1 steps behind it
@@ -282,6 +288,9 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     char* const here = lds + (t & (S - 1)) * STAGE;
     const char* const there = lds + ((t + 1) & (S - 1)) * STAGE;
     const unsigned next = (unsigned)(first + (t < last ? t + 1 : last)), sx_at = next * (unsigned)g.M;
+    if constexpr (EXACT)
+#pragma unroll
+      for (int i = 0; i < WTM; ++i) sx_now[i] = sx[i];  // (sx becomes the next step's during the last row of instructions)
 #pragma unroll
     for (int j = 0; j < WTN; ++j) {
       if (j == JB) {
@@ -298,12 +307,19 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
         if constexpr (EXACT) {
           if (i == 0)
 #pragma unroll
-            for (int h = 0; h < 4; ++h) WW[h] = widen(W[j % RING], h, scale_of(sw));
+            for (int h = 0; h < 4; ++h) WW[h] = widen(W[j % RING], h);
           if (j == 0)
 #pragma unroll
-            for (int h = 0; h < 4; ++h) XW[i][h] = widen(X[i], h, scale_of(sx[i]));
+            for (int h = 0; h < 4; ++h) XW[i][h] = widen(X[i], h);
+          // this block's sums from zero; they are scaled and added under the next fragments' instructions
+          f32x4& now = part[(j * WTM + i) & 1];
+          now = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int h = 0; h < 4; ++h) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(WW[h], XW[i][h], acc[j][i], 0, 0, 0);
+          for (int h = 0; h < 4; ++h) now = __builtin_amdgcn_mfma_f32_16x16x32_bf16(WW[h], XW[i][h], now, 0, 0, 0);
+          if (j * WTM + i > 0) {
+            const int before = j * WTM + i - 1;
+            add_scaled(acc[before / WTM][before % WTM], part[before & 1], sx_now[before % WTM], sw);
+          }
         } else {
           acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, sw, 0, sx[i]);
         }
@@ -340,6 +356,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if constexpr (EXACT) add_scaled(acc[WTN - 1][WTM - 1], part[(WTN * WTM - 1) & 1], sx_now[WTM - 1], sw);
     sw = sw_next;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no copy may land once this workgroup's shared memory is another's)
@@ -379,10 +396,10 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Few rows (up to 16 MT): the weights are streamed once and bound the time, so one launch does it all.  A workgroup owns
-// 16 NT channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as
-// fragments straight from memory, the next block's in flight, and brings the rows to 8 bits in registers - the four lanes that
-// hold a row's block find its largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
+// Few rows (up to 16): the weights are streamed once and bound the time.  A workgroup owns 16 channels, its waves share the
+// blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
+// block's in flight, and brings plain rows to 8 bits in registers - the four lanes that hold a row's block find its
+// largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
 // ---------------------------------------------------------------------------------------------------
 // 32 values of a row: columns k0 .. k0 + 15 and k0 + 64 .. k0 + 79, zeros behind K
 template <int DT>
@@ -430,93 +447,64 @@ struct FewRows {
   bool wide;
 };
 
-template <int DT, bool EXACT, int MT, int NT>
+template <int DT, bool EXACT>
 __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  f32x4* const sums = (f32x4*)smem;  // [wave][NT][MT][64]
+  __shared__ f32x4 sums[16][64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
-  const long n0 = (long)blockIdx.x * 16 * NT, pitch = (long)g.kb * FP8_BLOCK;
-  const uint8_t* w_row[NT];
-  const uint8_t* ws_row[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const long n = n0 + j * 16 + fr < g.N ? n0 + j * 16 + fr : g.N - 1;  // (channels past the end repeat the last, unstored)
-    w_row[j] = g.wq + n * pitch + fq * 16;
-    ws_row[j] = g.ws + (n >> 7) * g.kb;
-  }
-  f32x4 acc[NT][MT] = {};
-  i32x4 w_next[NT][2];
-  int sw_next[NT];
+  const long n0 = (long)blockIdx.x * 16, pitch = (long)g.kb * FP8_BLOCK;
+  const long nf = n0 + fr < g.N ? n0 + fr : g.N - 1;  // (channels and rows past the end repeat one that is there, unstored)
+  const bool on = fr < g.M;
+  const long mf = on ? fr : 0;
+  const uint8_t* const w_row = g.wq + nf * pitch + fq * 16;
+  const uint8_t* const ws_row = g.ws + (nf >> 7) * g.kb;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  i32x4 w_next[2];
+  int sw_next;
   auto fetch = [&](int b) {
     if (b >= g.kb) return;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      w_next[j][0] = *(const i32x4*)(w_row[j] + (long)b * FP8_BLOCK);
-      w_next[j][1] = *(const i32x4*)(w_row[j] + (long)b * FP8_BLOCK + 64);
-      sw_next[j] = ws_row[j][b];
-    }
+    w_next[0] = *(const i32x4*)(w_row + (long)b * FP8_BLOCK);
+    w_next[1] = *(const i32x4*)(w_row + (long)b * FP8_BLOCK + 64);
+    sw_next = ws_row[b];
   };
   fetch(wid);
   for (int b = wid; b < g.kb; b += waves) {
-    i32x8 W[NT], X[MT];
-    int sw[NT], sx[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const long m = i * 16 + fr;
-      const bool on = m < g.M;
-      if constexpr (DT == DT_E4M3) {
-        const uint8_t* q = (const uint8_t*)r.x + (on ? m : 0) * pitch + (long)b * FP8_BLOCK + fq * 16;
-        X[i] = __builtin_shufflevector(*(const i32x4*)q, *(const i32x4*)(q + 64), 0, 1, 2, 3, 4, 5, 6, 7);
-        sx[i] = r.x_scale[(on ? m : 0) * g.kb + b];
-      } else {
-        RowPart<DT> part;
-        part.load(r.x, (on ? m : 0) * r.row_stride, (long)b * FP8_BLOCK + fq * 16, r.K, on, r.wide);
-        sx[i] = part.quantise(X[i]);
-      }
+    i32x8 X;
+    int sx;
+    if constexpr (DT == DT_E4M3) {
+      const uint8_t* q = (const uint8_t*)r.x + mf * pitch + (long)b * FP8_BLOCK + fq * 16;
+      X = __builtin_shufflevector(*(const i32x4*)q, *(const i32x4*)(q + 64), 0, 1, 2, 3, 4, 5, 6, 7);
+      sx = r.x_scale[mf * g.kb + b];
+    } else {
+      RowPart<DT> part;
+      part.load(r.x, mf * r.row_stride, (long)b * FP8_BLOCK + fq * 16, r.K, on, r.wide);
+      sx = part.quantise(X);
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      W[j] = __builtin_shufflevector(w_next[j][0], w_next[j][1], 0, 1, 2, 3, 4, 5, 6, 7);
-      sw[j] = sw_next[j];
-    }
+    const i32x8 W = __builtin_shufflevector(w_next[0], w_next[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    const int sw = sw_next;
     fetch(b + waves);
+    if constexpr (EXACT) {
+      f32x4 part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if constexpr (EXACT) {
-        bf16x8 ww[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) ww[h] = widen(W[j], h, scale_of(sw[j]));
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 4; ++h) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[h], widen(X[i], h, scale_of(sx[i])), acc[j][i], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j], X[i], acc[j][i], 0, 0, 0, sw[j], 0, sx[i]);
-      }
+      for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(W, h), widen(X, h), part, 0, 0, 0);
+      add_scaled(acc, part, sx, sw);
+    } else {
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W, X, acc, 0, 0, 0, sw, 0, sx);
     }
   }
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sums[((wid * NT + j) * MT + i) * 64 + lane] = acc[j][i];
+  sums[wid][lane] = acc;
   __syncthreads();
-  for (int at = tid; at < NT * MT * 64; at += (int)blockDim.x) {
-    f32x4 v = sums[at];
-    for (int w = 1; w < waves; ++w) v += sums[w * NT * MT * 64 + at];
-    const int l = at & 63, i = (at >> 6) % MT, j = (at >> 6) / MT;
-    const long m = i * 16 + (l & 15), n = n0 + j * 16 + (l >> 4) * 4;
-    if (m >= g.M) continue;
+  if (tid >= 64 || !on) return;
+  for (int w = 1; w < waves; ++w) acc += sums[w][lane];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (n + e >= g.N) break;
-      const float y = v[e] + (g.bias ? g.bias[n + e] : 0.f);
-      const long o = m * g.N + n + e;
-      if constexpr (EXACT) ((float*)g.out)[o] = y;
-      else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)y;
-      else ((_Float16*)g.out)[o] = (_Float16)y;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const long n = n0 + fq * 4 + e;
+    if (n >= g.N) break;
+    const float y = acc[e] + (g.bias ? g.bias[n] : 0.f);
+    const long o = fr * g.N + n;
+    if constexpr (EXACT) ((float*)g.out)[o] = y;
+    else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)y;
+    else ((_Float16*)g.out)[o] = (_Float16)y;
   }
 }
 
@@ -605,21 +593,46 @@ hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride,
   return hipGetLastError();
 }
 
-// How a product is cut: the tile (in units of 32 rows and channels), and the pieces of its K loop.
+// How a product is cut: tiles of 32 `size` x 32 `size`, and the pieces of its K loop.
 struct Plan {
-  int wtm, wtn, parts;
+  int size, parts;
 };
+// The cheapest by what was measured of the tiles (microseconds).  A step of K takes a tile no less than `step` alone on its CU (its
+// latency), all tiles at work together no less than their copies take at 16 GB/ms of L2 and their products at `rate`; a round of
+// tiles has 2 to 3 us of start and end, and its results to write.  A cut K loop adds a launch and its sums' way through
+// memory.  Sides measured: 16384 x 1280 x 1280 256-tiles 47 us, 128-tiles 41; 4096^3 57 and 73; 512 x 8192 x 8192 128-tiles
+// 46, 64-tiles 59; 1024 x 1280 x 1280 12.1 and 11.2; 128 x 8192 x 8192 64-tiles whole 28.6, K cut in two 25.5.
 static Plan plan_of(int64_t M, int64_t N, int kb, bool exact) {
-  static const char* force = getenv("FT");
-  if (force) {
-    int a, b, c;
-    sscanf(force, "%d,%d,%d", &a, &b, &c);
-    return Plan{a, b, c < kb ? c : kb};
+  struct Kind {
+    int size, resident;
+    double step;
+  };
+  static const Kind fast[3] = {{8, 1, 1.1}, {4, 2, 0.6}, {2, 2, 0.24}}, wide[2] = {{4, 2, 1.55}, {2, 2, 0.75}};
+  const double rate = exact ? 0.75e9 : 2.6e9, l2 = 16e6, hbm = 4.5e6;  // per microsecond
+  Plan best{2, 1};
+  double least = 1e30;
+  for (int k = 0; k < (exact ? 2 : 3); ++k) {
+    const Kind& t = exact ? wide[k] : fast[k];
+    const double edge = 32.0 * t.size, slots = 256.0 * t.resident;
+    const double whole = (double)((M + 32 * t.size - 1) / (32 * t.size)) * (double)((N + 32 * t.size - 1) / (32 * t.size));
+    for (int parts = 1; parts <= 16; parts *= 2) {
+      if (parts > 1 && (kb < 4 * parts || whole * parts > 1024)) break;
+      const double work = whole * parts, steps = (double)((kb + parts - 1) / parts);
+      auto round = [&](double n) {
+        if (n <= 0) return 0.0;
+        const double step = std::max({t.step, n * 2 * edge * 128 / l2, n * edge * edge * 256 / rate});
+        return steps * step + (t.resident > 1 ? 2.0 : 3.0) + n * edge * edge * (parts > 1 || exact ? 4 : 2) / hbm / t.resident;
+      };
+      const double full = std::floor(work / slots);
+      double cost = full * round(slots) + round(work - full * slots);
+      if (parts > 1) cost += 4.0 + (double)M * N * (4.0 * parts + 4) / hbm;
+      if (cost < least) {
+        least = cost;
+        best = Plan{t.size, parts};
+      }
+    }
   }
-  const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-  if (big >= 200 && !exact) return Plan{8, 8, 1};
-  if (M > 64) return Plan{4, 4, 1};
-  return Plan{2, 2, 1};
+  return best;
 }
 
 template <int WTM, int WTN, int S, int OUT_DT, bool EXACT>
@@ -633,32 +646,23 @@ static hipError_t launch_tile(const Fp8Gemm& g, int parts, hipStream_t stream) {
 template <int OUT_DT, bool EXACT>
 static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t stream) {
   if constexpr (!EXACT) {
-    if (p.wtm == 8) return launch_tile<8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
+    if (p.size == 8) return launch_tile<8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
   }
-  if (p.wtm == 5) return launch_tile<4, 4, 4, OUT_DT, EXACT>(g, p.parts, stream);
-  if (p.wtm == 4) return launch_tile<4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
+  if (p.size == 4) return launch_tile<4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
   return launch_tile<2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
 }
 
-constexpr int FEW_ROWS = 32;
+constexpr int FEW_ROWS = 16;
+// Plain rows are brought to 8 bits inside that kernel up to this many blocks of K (every workgroup does it again: 8 x 2560 x
+// 2560 7.6 us against 10.3 us with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3).
+constexpr int FEW_BLOCKS = 24;
 
-template <int DT, bool EXACT, int MT>
-static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
-  // Waves share K: up to 16, none without a block.  Two channel fragments a wave where that still gives every CU a workgroup (the
-  // rows are brought to 8 bits once for them), else one.
-  const int waves = g.kb < 16 ? g.kb : 16;
-  const bool two = (g.N + 31) / 32 >= 256;
-  const int nt = two ? 2 : 1;
-  const dim3 grid((unsigned)((g.N + 16 * nt - 1) / (16 * nt)));
-  const size_t smem = (size_t)waves * nt * MT * 1024;
-  if (two) hipLaunchKernelGGL((few_rows_kernel<DT, EXACT, MT, 2>), grid, dim3(64 * waves), smem, stream, g, r);
-  else hipLaunchKernelGGL((few_rows_kernel<DT, EXACT, MT, 1>), grid, dim3(64 * waves), smem, stream, g, r);
-  return hipGetLastError();
-}
 template <int DT>
 static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
-  if (g.out_dt == DT_FP32) return g.M <= 16 ? launch_few_rows<DT, true, 1>(g, r, stream) : launch_few_rows<DT, true, 2>(g, r, stream);
-  return g.M <= 16 ? launch_few_rows<DT, false, 1>(g, r, stream) : launch_few_rows<DT, false, 2>(g, r, stream);
+  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
+  if (g.out_dt == DT_FP32) hipLaunchKernelGGL((few_rows_kernel<DT, true>), grid, block, 0, stream, g, r);
+  else hipLaunchKernelGGL((few_rows_kernel<DT, false>), grid, block, 0, stream, g, r);
+  return hipGetLastError();
 }
 
 template <int OUT_DT>
@@ -682,8 +686,8 @@ static int64_t scales_end(int64_t M, int64_t kb, bool quantised) {
   return (M * kb * (quantised ? 1 : FP8_BLOCK + 1) + 15) / 16 * 16;
 }
 int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact) {
-  if (M <= FEW_ROWS) return 0;
   const int64_t kb = fp8_blocks(K);
+  if (M <= FEW_ROWS) return quantised || kb <= FEW_BLOCKS ? 0 : M * kb * (FP8_BLOCK + 1);
   const Plan p = plan_of(M, N, (int)kb, exact);
   return scales_end(M, kb, quantised) + (p.parts > 1 ? p.parts * M * N * 4 : 0);
 }
@@ -692,10 +696,20 @@ hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   const int kb = (int)fp8_blocks(p.K);
   if (p.M <= FEW_ROWS) {
     const Fp8Gemm g{nullptr, nullptr, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
-    const FewRows r{p.x, (long)p.row_stride, (long)p.K, p.x_scale, p.x_dt != DT_E4M3 && wide_rows(p.x, p.x_dt, p.row_stride)};
-    if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, stream);
-    if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, stream);
-    if (p.x_dt == DT_FP16) return launch_few_rows<DT_FP16>(g, r, stream);
+    FewRows r{p.x, (long)p.row_stride, (long)p.K, p.x_scale, p.x_dt != DT_E4M3 && wide_rows(p.x, p.x_dt, p.row_stride)};
+    if (p.x_dt != DT_E4M3) {
+      if (kb <= FEW_BLOCKS) {
+        if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, stream);
+        if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, stream);
+        return launch_few_rows<DT_FP16>(g, r, stream);
+      }
+      uint8_t* const q = (uint8_t*)p.workspace;
+      uint8_t* const scale = q + p.M * kb * FP8_BLOCK;
+      const hipError_t e = quantize_rows<false>(p.x, p.x_dt, p.row_stride, p.M, p.K, q, scale, stream);
+      if (e != hipSuccess) return e;
+      r.x = q;
+      r.x_scale = scale;
+    }
     return launch_few_rows<DT_E4M3>(g, r, stream);
   }
   const uint8_t* xq = (const uint8_t*)p.x;
