@@ -8,7 +8,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # $EVODIFF_AMD_LIB: another build of the same library (A/B comparisons of kernel changes on one GPU box)
 LIB_PATH = os.environ.get("EVODIFF_AMD_LIB") or os.path.join(_HERE, "csrc", "libevodiff_hip.so")
 
-PREC_FP32, PREC_BF16 = 0, 1
+PREC_FP32, PREC_BF16, PREC_FP8 = 0, 1, 2
 DT_FP32, DT_BF16, DT_FP16, DT_E4M3 = 0, 1, 2, 3
 TOP_K_MAX = 32
 K_EMBED, K_LNACT, K_GEMM1X1, K_CONV, K_FINAL, K_CONV_OTHER, K_COUNT = 0, 1, 2, 3, 4, 5, 6

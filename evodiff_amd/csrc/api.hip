@@ -107,6 +107,13 @@ struct ed_model {
   // workspace
   int ws_B = 0, ws_L = 0, ws_prec = -1;
   DevBuf score_logits, score_ws;  // ed_score_tokens
+  // ED_PREC_FP8: the three matrices of every layer in 8 bits (made from the fp32 image at the first call that needs them), and the
+  // operands of a layer: rows, and the convolution's padded rows, each with their scales.
+  struct LayerW8 { const uint8_t *w1, *s1, *wc, *sc, *w2, *s2; };
+  DevBuf w8, a8, c8;
+  std::vector<LayerW8> layers8;
+  bool packed8 = false;
+  int c8_B = 0, c8_L = 0;
   DevBuf X, X2, Abuf, Ybuf, Cpad, Cprune, state, tok, order, uni, qbuf, tvec;
   // Incremental leading layers (OA-DM, ED_OPT_INCREMENTAL): between two steps ONE token per sequence changes, so
   // layer k only changes within r_k = r_{k-1} + 2 d_k positions of it.  The first n_inc layers keep their outputs
@@ -724,12 +731,109 @@ int run_embed(ed_model* m, const int64_t* tokens, const int64_t* tvec, int B, in
   return ED_OK;
 }
 
-int check_shape(const ed_model* m, int B, int L, int prec) {
+// fp8: the entry point takes ED_PREC_FP8 too
+int check_shape(const ed_model* m, int B, int L, int prec, bool fp8 = false) {
   if (!m) return fail(ED_EINVAL, "null model handle");
   if (!m->committed) return fail(ED_ESTATE, "ed_model_commit has not been called");
   if (B <= 0 || L <= 0) return fail(ED_EINVAL, "B and L must be positive (got B=%d L=%d)", B, L);
   if ((int64_t)B * L > (1 << 30)) return fail(ED_EINVAL, "B*L too large");
-  if (prec != ED_PREC_FP32 && prec != ED_PREC_BF16) return fail(ED_EINVAL, "unknown precision %d", prec);
+  if (prec == ED_PREC_FP8 && !fp8) return fail(ED_EINVAL, "ED_PREC_FP8 is for ed_forward and the scoring entry points; the sampling loops run in fp32 or bf16");
+  if (prec != ED_PREC_FP32 && prec != ED_PREC_BF16 && prec != ED_PREC_FP8) return fail(ED_EINVAL, "unknown precision %d", prec);
+  return ED_OK;
+}
+
+// ---- ED_PREC_FP8 ----
+// Weights in 8 bits, one scale for 128 x 128 values (a convolution's taps lie side by side in a row).
+int ensure_packed8(ed_model* m, hipStream_t s) {
+  if (m->packed8) return ED_OK;
+  const ed_config& c = m->cfg;
+  const int64_t D = c.d_model, H = c.d_hidden, KS = c.kernel_size, kd = fp8_blocks(D), kh = fp8_blocks(H);
+  auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
+  const int64_t w1 = up(H * kd * FP8_BLOCK), s1 = up(fp8_blocks(H) * kd), wc = up(H * KS * kh * FP8_BLOCK), sc = up(fp8_blocks(H) * KS * kh),
+                w2 = up(D * kh * FP8_BLOCK), s2 = up(fp8_blocks(D) * kh), layer = w1 + s1 + wc + sc + w2 + s2;
+  HIP_TRY(m->w8.ensure((size_t)(layer * c.n_layers)));
+  m->layers8.resize((size_t)c.n_layers);
+  for (int i = 0; i < c.n_layers; ++i) {
+    uint8_t* p = m->w8.as<uint8_t>() + layer * i;
+    ed_model::LayerW8& w = m->layers8[(size_t)i];
+    w.w1 = p; w.s1 = w.w1 + w1; w.wc = w.s1 + s1; w.sc = w.wc + wc; w.w2 = w.sc + sc; w.s2 = w.w2 + w2;
+    const LayerW& f = m->layers[(size_t)i];
+    LAUNCH_TRY(launch_fp8_quantize_weight(f.w1_f, DT_FP32, D, H, D, (uint8_t*)w.w1, (uint8_t*)w.s1, s));
+    LAUNCH_TRY(launch_fp8_quantize_weight(f.w2_f, DT_FP32, H, D, H, (uint8_t*)w.w2, (uint8_t*)w.s2, s));
+    for (int64_t t = 0; t < KS; ++t)
+      LAUNCH_TRY(launch_fp8_quantize_weight(f.wc_f + t * H * H, DT_FP32, H, H, H, (uint8_t*)w.wc, (uint8_t*)w.sc, s, (int)(KS * kh), (int)(t * kh)));
+  }
+  HIP_TRY(hipStreamSynchronize(s));  // (once: calls on other streams may follow)
+  m->packed8 = true;
+  return ED_OK;
+}
+
+// The block stack with every product in 8 bits: each LayerNorm writes its GELU straight into blocks of 128 for the product behind it;
+// products leave bf16 (PFF1, convolution) or add to the fp32 residual stream (PFF2).  X holds the embedded rows.
+int run_blocks_fp8(ed_model* m, int B, int L, float* acts, hipStream_t s) {
+  const ed_config& c = m->cfg;
+  const int D = c.d_model, H = c.d_hidden, rows = B * L, act = c.activation == 1 ? 1 : 2, kd = (int)fp8_blocks(D), kh = (int)fp8_blocks(H);
+  if (int rc = ensure_packed8(m, s)) return rc;
+  int max_dil = 1;
+  for (const auto& w : m->layers) max_dil = std::max(max_dil, w.dilation);
+  const int center = c.causal ? c.kernel_size - 1 : c.kernel_size / 2;
+  const long halo = (long)center * max_dil, pitch = L + halo, c_rows = (long)B * pitch + halo;  // zero rows in front, between and behind
+  const int64_t kmax = std::max(kd, kh);
+  if (c_rows * kh >= (1LL << 25)) return fail(ED_EINVAL, "ED_PREC_FP8: B*L too large");  // (rows are addressed with 32 bits)
+  HIP_TRY(m->a8.ensure((size_t)(rows * kmax * (FP8_BLOCK + 1))));
+  const size_t cbytes = (size_t)(c_rows * kh * (FP8_BLOCK + 1));
+  if (cbytes > m->c8.bytes || m->c8_B != B || m->c8_L != L) {  // (another layout: other rows are the zero ones)
+    HIP_TRY(m->c8.ensure(cbytes));
+    HIP_TRY(hipMemsetAsync(m->c8.p, 0, m->c8.bytes, s));
+    m->c8_B = B;
+    m->c8_L = L;
+  }
+  uint8_t* const a = m->a8.as<uint8_t>();
+  uint8_t* const cq = m->c8.as<uint8_t>();
+  uint8_t* const cs = cq + c_rows * kh * FP8_BLOCK;
+  float* const X = m->X.as<float>();
+  bf16_t* const Y = m->Ybuf.as<bf16_t>();
+  auto ln = [&](const void* in, bool bf, const float* g, const float* b, int C, uint8_t* q, uint8_t* sc, long q_rows, int seq, long sp, long r0) -> int {
+    Probe pr(m, s);
+    LAUNCH_TRY(pr.begin());
+    LAUNCH_TRY(launch_ln_act_fp8(in, bf, g, b, rows, C, act, q, sc, q_rows, seq, sp, r0, s));
+    LAUNCH_TRY(pr.end(ED_K_LNACT, 0.0, (double)rows * C * (bf ? 3.0 : 5.0)));
+    return ED_OK;
+  };
+  auto gemm = [&](const Fp8Gemm& g, int kind) -> int {
+    Probe pr(m, s);
+    LAUNCH_TRY(pr.begin());
+    LAUNCH_TRY(launch_fp8_gemm(g, s));
+    double taps = 0;
+    for (int t = 0; t < g.ntaps; ++t) taps += std::max(0.0, 1.0 - std::fabs((double)(t - g.center) * g.dilation) / L);
+    LAUNCH_TRY(pr.end(kind, 2.0 * rows * taps * g.N * g.kb * FP8_BLOCK,
+                      (double)rows * g.kb * FP8_BLOCK + (double)g.N * g.ntaps * g.kb * FP8_BLOCK + (double)rows * g.N * (g.resid ? 8.0 : 2.0)));
+    return ED_OK;
+  };
+  for (int i = 0; i < c.n_layers; ++i) {
+    const LayerW& w = m->layers[(size_t)i];
+    const ed_model::LayerW8& q = m->layers8[(size_t)i];
+    uint8_t* as = a + (long)rows * kd * FP8_BLOCK;
+    int rc;
+    if ((rc = ln(X, false, w.ln1_g, w.ln1_b, D, a, as, rows, rows, rows, 0))) return rc;
+    if ((rc = gemm(Fp8Gemm{a, as, q.w1, q.s1, w.b1, Y, DT_BF16, rows, H, kd}, ED_K_GEMM1X1))) return rc;
+    if ((rc = ln(Y, true, w.ln2_g, w.ln2_b, H, cq, cs, c_rows, L, pitch, halo))) return rc;
+    Fp8Gemm conv{cq, cs, q.wc, q.sc, w.bc, Y, DT_BF16, rows, H, kh};
+    conv.ntaps = c.kernel_size;
+    conv.dilation = w.dilation;
+    conv.center = center;
+    conv.L = L;
+    conv.x_seq_pitch = pitch;
+    conv.x_row0 = halo;
+    conv.x_rows = c_rows;
+    if ((rc = gemm(conv, c.kernel_size > 1 ? ED_K_CONV_OTHER : ED_K_GEMM1X1))) return rc;
+    as = a + (long)rows * kh * FP8_BLOCK;
+    if ((rc = ln(Y, true, w.ln3_g, w.ln3_b, H, a, as, rows, rows, rows, 0))) return rc;
+    Fp8Gemm out{a, as, q.w2, q.s2, w.b2, X, DT_FP32, rows, D, kh};
+    out.resid = X;
+    if ((rc = gemm(out, ED_K_GEMM1X1))) return rc;
+    if (acts) HIP_TRY(hipMemcpyAsync(acts + (size_t)(i + 1) * rows * D, X, (size_t)rows * D * 4, hipMemcpyDeviceToDevice, s));
+  }
   return ED_OK;
 }
 
@@ -1075,6 +1179,7 @@ int ed_model_commit(ed_model* m) {
     HIP_TRY(hipDeviceSynchronize());
   }
   m->staged.clear();
+  m->packed8 = false;
   m->drop_graphs();
   m->committed = true;
   return ED_OK;
@@ -1090,14 +1195,14 @@ int ed_model_get_config(const ed_model* m, ed_config* out) {
 
 int ed_forward_collect(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_dev, int B, int L,
                        float* logits_dev, float* acts_dev, int precision, void* stream) {
-  int rc = check_shape(m, B, L, precision);
+  int rc = check_shape(m, B, L, precision, true);
   if (rc) return rc;
   if (!tokens_dev || !logits_dev) return fail(ED_EINVAL, "null tokens/logits pointer");
   if (m->cfg.timesteps > 0 && !timesteps_dev) return fail(ED_EINVAL, "timesteps_dev is required for a model with timestep encoding");
   hipStream_t s = (hipStream_t)stream;
   HIP_TRY(hipSetDevice(m->device));
   if ((rc = check_async_errors(m))) return rc;
-  if ((rc = ensure_workspace(m, B, L, precision, s))) return rc;
+  if ((rc = ensure_workspace(m, B, L, precision == ED_PREC_FP8 ? ED_PREC_BF16 : precision, s))) return rc;
   // range checks on the device (clamp + asynchronous report): the kernels read the model's own, clamped copies
   LAUNCH_TRY(launch_prepare_ids(tokens_dev, m->tok.as<int64_t>(), (long)B * L, m->cfg.n_tokens, m->ln_err_dev, ED_AERR_TOKEN, s));
   if (m->cfg.timesteps > 0)
@@ -1106,7 +1211,7 @@ int ed_forward_collect(ed_model* m, const int64_t* tokens_dev, const int64_t* ti
   rc = run_embed(m, m->tok.as<int64_t>(), m->cfg.timesteps > 0 ? m->tvec.as<int64_t>() : nullptr, B, L, STEP_PLAIN, s);
   if (!rc && acts_dev)
     HIP_TRY(hipMemcpyAsync(acts_dev, m->X.p, (size_t)B * L * m->cfg.d_model * 4, hipMemcpyDeviceToDevice, s));
-  if (!rc) rc = run_blocks(m, B, L, precision, acts_dev, false, STEP_PLAIN, nullptr, s);
+  if (!rc) rc = precision == ED_PREC_FP8 ? run_blocks_fp8(m, B, L, acts_dev, s) : run_blocks(m, B, L, precision, acts_dev, false, STEP_PLAIN, nullptr, s);
   if (!rc) {
     Probe pr(m, s);
     LAUNCH_TRY(pr.begin());
@@ -1125,7 +1230,7 @@ int ed_forward(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_
 
 int ed_score_nll(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_dev, const int64_t* targets_dev,
                  const uint8_t* select_dev, int B, int L, int n_classes, float* nll_dev, int precision, void* stream) {
-  int rc = check_shape(m, B, L, precision);
+  int rc = check_shape(m, B, L, precision, true);
   if (rc) return rc;
   if (!tokens_dev || !targets_dev || !nll_dev) return fail(ED_EINVAL, "null tokens/targets/nll pointer");
   if (m->cfg.timesteps > 0 && !timesteps_dev) return fail(ED_EINVAL, "timesteps_dev is required for a model with timestep encoding");
@@ -1133,7 +1238,7 @@ int ed_score_nll(ed_model* m, const int64_t* tokens_dev, const int64_t* timestep
   hipStream_t s = (hipStream_t)stream;
   HIP_TRY(hipSetDevice(m->device));
   if ((rc = check_async_errors(m))) return rc;
-  if ((rc = ensure_workspace(m, B, L, precision, s))) return rc;
+  if ((rc = ensure_workspace(m, B, L, precision == ED_PREC_FP8 ? ED_PREC_BF16 : precision, s))) return rc;
   // range checks on the device (clamp + asynchronous report; the scoring tail clamps the targets itself)
   LAUNCH_TRY(launch_prepare_ids(tokens_dev, m->tok.as<int64_t>(), (long)B * L, m->cfg.n_tokens, m->ln_err_dev, ED_AERR_TOKEN, s));
   if (m->cfg.timesteps > 0)
@@ -1141,7 +1246,7 @@ int ed_score_nll(ed_model* m, const int64_t* tokens_dev, const int64_t* timestep
   LAUNCH_TRY(launch_check_targets(targets_dev, select_dev, (long)B * L, n_classes, m->ln_err_dev, s));
   m->probing_now = m->probe_every > 0;
   rc = run_embed(m, m->tok.as<int64_t>(), m->cfg.timesteps > 0 ? m->tvec.as<int64_t>() : nullptr, B, L, STEP_PLAIN, s);
-  if (!rc) rc = run_blocks(m, B, L, precision, nullptr, false, STEP_PLAIN, nullptr, s);
+  if (!rc) rc = precision == ED_PREC_FP8 ? run_blocks_fp8(m, B, L, nullptr, s) : run_blocks(m, B, L, precision, nullptr, false, STEP_PLAIN, nullptr, s);
   if (!rc) {
     Probe pr(m, s);
     LAUNCH_TRY(pr.begin());
@@ -1697,7 +1802,7 @@ int ed_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row_st
 int ed_score_tokens(ed_model* m, const int64_t* tokens_dev, const int64_t* timesteps_dev, const int64_t* targets_dev,
                     const uint8_t* select_dev, int B, int L, int n_classes, int top_k, float* logprob_dev,
                     float* entropy_dev, float* top_logprob_dev, int64_t* top_token_dev, int precision, void* stream) {
-  int rc = check_shape(m, B, L, precision);
+  int rc = check_shape(m, B, L, precision, true);
   if (rc) return rc;
   if (!targets_dev || !logprob_dev || !entropy_dev) return fail(ED_EINVAL, "null targets/logprob/entropy pointer");
   const int V = m->cfg.n_tokens;

@@ -3,6 +3,8 @@
 // All are HBM-bound: one 64-lane wave owns one row, loads are 16 bytes (fp32) / 8 bytes (bf16) per lane,
 // statistics are reduced with cross-lane shuffles, nothing is staged through LDS except small tables.
 #include "kernels.hpp"
+#include "fp8_block.hpp"
+#include "ops.hpp"
 
 #include <type_traits>
 
@@ -359,6 +361,88 @@ __global__ __launch_bounds__(256) void ln_act_fast_kernel(const void* __restrict
       const bf16x4 pk = {(__bf16)v[k], (__bf16)v[k + 1], (__bf16)v[k + 2], (__bf16)v[k + 3]};
       *(bf16x4*)(dst + chan(k)) = pk;
     }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// LayerNorm + activation into blocks of 128 in 8 bits (ED_PREC_FP8): one pass, bound by HBM (a 1280-channel row in bf16 is 2.5 KB
+// in, 1.3 KB out).  A wave owns a row, 8 neighbouring channels a lane and chunk of 512, so that 16 lanes hold a block; the
+// statistics are taken on the values in registers, mean first.
+// ---------------------------------------------------------------------------------------------------
+template <int NC8, bool IN_BF16, int ACT>
+__global__ __launch_bounds__(256) void ln_act_fp8_kernel(const void* __restrict__ in, const float* __restrict__ gamma,
+                                                         const float* __restrict__ beta, int rows, int C, uint8_t* __restrict__ q,
+                                                         uint8_t* __restrict__ scale, long q_rows, int L, long seq_pitch, long row0) {
+  const int lane = threadIdx.x & 63;
+  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  if (row >= rows) return;
+  const int seq = row / L;
+  const long orow = (long)seq * seq_pitch + row0 + (row - seq * L);
+  float v[NC8][8];
+#pragma unroll
+  for (int c = 0; c < NC8; ++c) {
+    const int k = c * 512 + lane * 8;
+    if (k < C) {  // (C is a multiple of 8)
+      if constexpr (IN_BF16) {
+        const uint4 raw = *(const uint4*)((const bf16_t*)in + (long)row * C + k);
+        const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[c][2 * j] = __uint_as_float(w[j] << 16);
+          v[c][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      } else {
+        const float4 a = *(const float4*)((const float*)in + (long)row * C + k), b = *(const float4*)((const float*)in + (long)row * C + k + 4);
+        v[c][0] = a.x; v[c][1] = a.y; v[c][2] = a.z; v[c][3] = a.w;
+        v[c][4] = b.x; v[c][5] = b.y; v[c][6] = b.z; v[c][7] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[c][j] = 0.f;
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC8; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += v[c][j];
+  const float mean = wave_sum_dpp(s) / (float)C;
+  float sq = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC8; ++c) {
+    const bool on = c * 512 + lane * 8 < C;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[c][j] = on ? v[c][j] - mean : 0.f;
+      sq = fmaf(v[c][j], v[c][j], sq);
+    }
+  }
+  const float rstd = rsqrtf(wave_sum_dpp(sq) / (float)C + LN_EPS);
+  const int kb = (C + 127) / 128;
+#pragma unroll
+  for (int c = 0; c < NC8; ++c) {
+    const int k = c * 512 + lane * 8, blk = k >> 7;
+    if (blk >= kb) continue;  // (whole groups of 16 lanes)
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float t = 0.f;
+      if (k < C) {
+        t = fmaf(v[c][j] * rstd, gamma[k + j], beta[k + j]);
+        if constexpr (ACT == 1) t = gelu_sigmoid_fit(t);
+        else if constexpr (ACT == 2) t = fmaxf(t, 0.f);
+      }
+      y[j] = t;
+    }
+    unsigned a = amax8(y);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const unsigned b = (unsigned)__shfl_xor((int)a, o);
+      a = b > a ? b : a;
+    }
+    const int byte = scale_byte(a);
+    *(uint2*)(q + (orow * kb + blk) * 128 + (k & 127)) = pack8(y, inverse_scale(byte));
+    if ((lane & 15) == 0) scale[(long)blk * q_rows + orow] = (uint8_t)byte;
   }
 }
 
@@ -936,6 +1020,30 @@ hipError_t launch_init_state(StepState* state, int step, int t_start, hipStream_
 
 hipError_t launch_advance_step(StepState* state, hipStream_t stream) {
   hipLaunchKernelGGL(advance_step_kernel, dim3(1), dim3(1), 0, stream, state);
+  return hipGetLastError();
+}
+
+hipError_t launch_ln_act_fp8(const void* in, bool in_bf16, const float* gamma, const float* beta, int rows, int C, int act, uint8_t* q,
+                             uint8_t* scale, long q_rows, int L, long seq_pitch, long row0, hipStream_t stream) {
+  if (C % 8 || C > 2048 || rows < 1) return hipErrorInvalidValue;
+  const dim3 grid((rows + 3) / 4), block(256);
+#define ED_GO(NC8, BF, ACT)                                                                                               \
+  hipLaunchKernelGGL((ln_act_fp8_kernel<NC8, BF, ACT>), grid, block, 0, stream, in, gamma, beta, rows, C, q, scale, q_rows, L, \
+                     seq_pitch, row0)
+#define ED_ACT(NC8, BF)                                                                                                   \
+  if (act == 1) ED_GO(NC8, BF, 1);                                                                                         \
+  else if (act == 2) ED_GO(NC8, BF, 2);                                                                                    \
+  else ED_GO(NC8, BF, 0)
+#define ED_CH(BF)                                                                                                         \
+  if (C <= 512) { ED_ACT(1, BF); }                                                                                         \
+  else if (C <= 1024) { ED_ACT(2, BF); }                                                                                   \
+  else if (C <= 1536) { ED_ACT(3, BF); }                                                                                   \
+  else { ED_ACT(4, BF); }
+  if (in_bf16) { ED_CH(true) }
+  else { ED_CH(false) }
+#undef ED_CH
+#undef ED_ACT
+#undef ED_GO
   return hipGetLastError();
 }
 

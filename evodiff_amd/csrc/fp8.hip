@@ -5,6 +5,7 @@
 // the small end), are exact to apply, and are what the matrix instruction takes beside its operands (E8M0 bytes): the
 // product needs no vector instruction for its scales.
 #include "ops.hpp"
+#include "fp8_block.hpp"
 
 #include <hip/hip_fp16.h>
 
@@ -27,13 +28,6 @@ struct Elem<DT_BF16> { typedef __bf16 T; };
 template <>
 struct Elem<DT_FP16> { typedef _Float16 T; };
 
-// E8M0 byte of the scale for a block whose largest magnitude has these bits: 448 = 2^8 * (1 + 0x600000 / 2^23).
-__device__ __forceinline__ int scale_byte(unsigned amax) {
-  const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < 1 ? 1 : e > 254 ? 254 : e;
-}
-__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }  // 2^(127 - byte)
-
 // Eight values of a row at column k0 (a multiple of 8): zeros behind K.
 template <int DT>
 __device__ __forceinline__ void load8(const typename Elem<DT>::T* row, long k0, long K, bool wide, float (&v)[8]) {
@@ -48,26 +42,6 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::T* row, long k0, 
     for (int i = 0; i < 8; ++i) v[i] = k0 + i < K ? (float)row[k0 + i] : 0.f;
   }
 }
-// largest magnitude (as bits) of eight values; Inf and NaN do not count and become NaN
-__device__ __forceinline__ unsigned amax8(float (&v)[8]) {
-  unsigned a = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
-    if (b >= 0x7f800000u) v[i] = __builtin_nanf("");
-    else a = b > a ? b : a;
-  }
-  return a;
-}
-__device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
-  uint2 r;
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
-  r.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
-  r.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, w, true);
-  return r;
-}
-
 // 16 lanes own a block of 128; a workgroup takes U blocks of 16 rows, all loads first.  TURNED: scales go to (kb, rows), as the
 // product reads them (16 rows' bytes side by side), instead of (rows, kb).
 template <int DT, int U, bool TURNED>
@@ -101,7 +75,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
 template <int DT>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __restrict__ w, long row_stride, long N, int kb,
                                                               long K, bool wide, uint8_t* __restrict__ q,
-                                                              uint8_t* __restrict__ scale) {
+                                                              uint8_t* __restrict__ scale, int kb_row, int b_first) {
   __shared__ unsigned red[4];
   const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const long nb = blockIdx.x / kb;
@@ -131,9 +105,9 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const long row = nb * FP8_BLOCK + r0 + i * 16;
-    if (row < N) *(uint2*)(q + (row * kb + b) * FP8_BLOCK + l * 8) = pack8(v[i], inv);
+    if (row < N) *(uint2*)(q + (row * kb_row + b_first + b) * FP8_BLOCK + l * 8) = pack8(v[i], inv);
   }
-  if (threadIdx.x == 0) scale[nb * kb + b] = (uint8_t)byte;
+  if (threadIdx.x == 0) scale[nb * kb_row + b_first + b] = (uint8_t)byte;
 }
 
 
@@ -198,7 +172,11 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 //
 // The channels of an LDS tile are permuted within 32 so that two instructions give a lane eight consecutive ones: 16-byte stores.
 // ---------------------------------------------------------------------------------------------------
-template <int WTM, int WTN, int S, int OUT_DT, bool EXACT>
+//
+// TAPS: the rows are positions of sequences and every one is multiplied from `ntaps` of them (a dilated convolution): K runs over
+// taps, then blocks; a tap moves the row operand by `dilation` rows of its padded layout, whose rows around a sequence hold
+// zeros.  Taps that move a whole tile outside its sequence are left out.
+template <int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS>
 __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
   constexpr int BM = 32 * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
   constexpr int GX = BM / 32, GW = BN / 32, NG = GX + GW;  // 8-row copies a wave makes of each operand
@@ -219,39 +197,79 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     tile_n = in / high;
     tile_m = 4 * band + in - tile_n * high;
   }
-  const long m0 = (long)tile_m * BM, n0 = (long)tile_n * BN, pitch = (long)g.kb * FP8_BLOCK;
+  const long m0 = (long)tile_m * BM, n0 = (long)tile_n * BN;
+  const long x_pitch = (long)g.kb * FP8_BLOCK;
+  const int kb_all = TAPS ? g.kb * g.ntaps : g.kb;  // blocks of a weight row
+  const long w_pitch = (long)kb_all * FP8_BLOCK;
   // blocks of K of this workgroup (never none: the launcher cuts into no more pieces than there are)
-  const int first = (int)((long)g.kb * blockIdx.y / gridDim.y), T = (int)((long)g.kb * (blockIdx.y + 1) / gridDim.y) - first;
+  int first = (int)((long)kb_all * blockIdx.y / gridDim.y), T = (int)((long)kb_all * (blockIdx.y + 1) / gridDim.y) - first;
+  // row of x that output row m reads at tap 0
+  auto x_row = [&](long m) -> long {
+    if constexpr (!TAPS) return m;
+    const unsigned seq = (unsigned)m / (unsigned)g.L, l = (unsigned)m - seq * (unsigned)g.L;
+    return (long)seq * g.x_seq_pitch + g.x_row0 + l - (long)g.center * g.dilation;
+  };
+  if constexpr (TAPS) {
+    const int l0 = (int)(m0 % g.L);
+    if (l0 + BM <= g.L) {  // the tile lies in one sequence
+      int lo = 0, hi = g.ntaps - 1;
+      while (lo < g.center && l0 + BM + (lo - g.center) * g.dilation <= 0) ++lo;
+      while (hi > g.center && l0 + (hi - g.center) * g.dilation >= g.L) --hi;
+      first = lo * g.kb;
+      T = (hi - lo + 1) * g.kb;
+    }
+  }
 
   // copies: lane -> (row of 8, physical chunk)
   const int chunk0 = ((lane & 7) ^ (lane >> 4)) * 16, chunk1 = ((lane & 7) ^ (4 + (lane >> 4))) * 16;
+  const long x_first = x_row(m0);
   unsigned off[NG];
 #pragma unroll
   for (int j = 0; j < GX; ++j) {
     const int row = (wid * GX + j) * 8 + (lane >> 3);
-    off[j] = (unsigned)(row * pitch) + ((wid * GX + j) & 1 ? chunk1 : chunk0);
+    const long m = TAPS && m0 + row >= g.M ? g.M - 1 : m0 + row;
+    off[j] = (unsigned)((x_row(m) - x_first) * x_pitch) + ((wid * GX + j) & 1 ? chunk1 : chunk0);
   }
 #pragma unroll
   for (int j = 0; j < GW; ++j) {
     const int lr = (wid * GW + j) * 8 + (lane >> 3);
     const int ch = (lr & ~31) + 8 * ((lr & 15) >> 2) + 4 * ((lr >> 4) & 1) + (lr & 3);
-    off[GX + j] = (unsigned)(ch * pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
+    off[GX + j] = (unsigned)(ch * w_pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
   }
-  const buffer_t x_src = buffer_of(g.xq + m0 * pitch, (g.M - m0) * pitch);
-  const buffer_t w_src = buffer_of(g.wq + n0 * pitch, (g.N - n0) * pitch);
+  const long x_rows = TAPS ? g.x_rows : g.M;
+  const buffer_t x_src = buffer_of(g.xq + x_first * x_pitch, (x_rows - x_first) * x_pitch);
+  const buffer_t w_src = buffer_of(g.wq + n0 * w_pitch, (g.N - n0) * w_pitch);
   // Past the last step the copies repeat its block (in bounds, into a stage nobody reads).
   const int last = T - 1;
   auto copy = [&](int j, int t, char* stage) {  // piece j of step t
-    const unsigned at = (unsigned)(first + (t < last ? t : last)) * FP8_BLOCK;
-    if (j < GX) copy16(x_src, off[j], at, stage + (wid * GX + j) * 1024);
-    else copy16(w_src, off[j], at, stage + BM * 128 + (wid * GW + j - GX) * 1024);
+    const unsigned b = (unsigned)(first + (t < last ? t : last));
+    if (j < GX) {
+      const unsigned tap = TAPS ? b / (unsigned)g.kb : 0;
+      const unsigned at = TAPS ? tap * (unsigned)g.dilation * (unsigned)x_pitch + (b - tap * (unsigned)g.kb) * FP8_BLOCK : b * FP8_BLOCK;
+      copy16(x_src, off[j], at, stage + (wid * GX + j) * 1024);
+    } else {
+      copy16(w_src, off[j], b * FP8_BLOCK, stage + BM * 128 + (wid * GW + j - GX) * 1024);
+    }
   };
 
   // scales: a lane's row in each of the WTM fragments; the wave's channels lie in one block of 128
-  const unsigned mw = (unsigned)(m0 + wr * 16 * WTM + fr);
+  unsigned sx_row[TAPS ? WTM : 1];
+  if constexpr (TAPS)
+#pragma unroll
+    for (int i = 0; i < WTM; ++i) {
+      const long m = m0 + wr * 16 * WTM + i * 16 + fr;
+      sx_row[i] = (unsigned)x_row(m < g.M ? m : g.M - 1);
+    }
+  else
+    sx_row[0] = (unsigned)(m0 + wr * 16 * WTM + fr);
   const long nw = n0 + wc * 16 * WTN;
-  const buffer_t sx_src = buffer_of(g.xs, g.M * (long)g.kb);  // (kb, M)
-  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * g.kb, g.kb);
+  const buffer_t sx_src = buffer_of(g.xs, x_rows * (long)g.kb);  // (kb, rows)
+  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * kb_all, kb_all);
+  auto row_scale = [&](int i, unsigned b) {  // of fragment i at block b
+    const unsigned tap = TAPS ? b / (unsigned)g.kb : 0;
+    const unsigned at = TAPS ? (b - tap * (unsigned)g.kb) * (unsigned)x_rows + tap * (unsigned)g.dilation : b * (unsigned)x_rows;
+    return load_byte(sx_src, TAPS ? sx_row[TAPS ? i : 0] : sx_row[0] + i * 16, at);
+  };
 
   const int swz = (fq ^ ((fr >> 1) & 7)) << 4;
   const int x_rd = (wr * 16 * WTM + fr) * 128, w_rd = BM * 128 + (wc * 16 * WTN + fr) * 128;
@@ -272,7 +290,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
 #pragma unroll
   for (int j = 0; j < NG; ++j) copy(j, 0, lds);
 #pragma unroll
-  for (int i = 0; i < WTM; ++i) sx[i] = load_byte(sx_src, mw + i * 16, (unsigned)first * (unsigned)g.M);
+  for (int i = 0; i < WTM; ++i) sx[i] = row_scale(i, (unsigned)first);
   sw = load_byte(sw_src, 0, (unsigned)first);
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
@@ -287,7 +305,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   for (int t = 0; t < T; ++t) {
     char* const here = lds + (t & (S - 1)) * STAGE;
     const char* const there = lds + ((t + 1) & (S - 1)) * STAGE;
-    const unsigned next = (unsigned)(first + (t < last ? t + 1 : last)), sx_at = next * (unsigned)g.M;
+    const unsigned next = (unsigned)(first + (t < last ? t + 1 : last));
     if constexpr (EXACT)
 #pragma unroll
       for (int i = 0; i < WTM; ++i) sx_now[i] = sx[i];  // (sx becomes the next step's during the last row of instructions)
@@ -332,7 +350,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
             if (want == slot) put(W[f % RING], r & 1, read(here, w_rd + f * 2048, r & 1));
           }
           constexpr int AT = JB * WTM >= 4 + WTM ? 4 : 0;  // the next step's scales
-          if (slot >= AT && slot < AT + WTM) sx_next[slot - AT] = load_byte(sx_src, mw + (slot - AT) * 16, sx_at);
+          if (slot >= AT && slot < AT + WTM) sx_next[slot - AT] = row_scale(slot - AT, next);
           if (slot == AT) sw_next = load_byte(sw_src, 0, next);
         } else {
           constexpr int COPY_SLOTS = (WTN - JB) * WTM;
@@ -381,6 +399,12 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     for (int J = 0; J < WTN / 2; ++J) {
       const long n = nw + 32 * J + 8 * fq;
       T_out* const to = out + m * g.N + n;
+      if constexpr (OUT_DT == DT_FP32 && !EXACT)
+        if (g.resid) {  // (may be the output: a lane reads what it writes)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < g.N) acc[2 * J + (e >> 2)][i][e & 3] += g.resid[m * g.N + n + e];
+        }
       if (wide && n + 8 <= g.N) {
         V8 v;
 #pragma unroll
@@ -581,11 +605,12 @@ hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, i
 }
 
 hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride, int64_t N, int64_t K, uint8_t* q,
-                                      uint8_t* scale, hipStream_t stream) {
+                                      uint8_t* scale, hipStream_t stream, int kb_row, int b_first) {
   const int kb = (int)fp8_blocks(K);
+  if (kb_row == 0) kb_row = kb;
   const dim3 grid((unsigned)(fp8_blocks(N) * kb));
   const bool wide = wide_rows(w, dt, row_stride);
-#define ED_GO(DT) hipLaunchKernelGGL((quantize_weight_kernel<DT>), grid, dim3(256), 0, stream, w, (long)row_stride, (long)N, kb, (long)K, wide, q, scale)
+#define ED_GO(DT) hipLaunchKernelGGL((quantize_weight_kernel<DT>), grid, dim3(256), 0, stream, w, (long)row_stride, (long)N, kb, (long)K, wide, q, scale, kb_row, b_first)
   if (dt == DT_FP32) ED_GO(DT_FP32);
   else if (dt == DT_BF16) ED_GO(DT_BF16);
   else ED_GO(DT_FP16);
@@ -602,7 +627,7 @@ struct Plan {
 // tiles has 2 to 3 us of start and end, and its results to write.  A cut K loop adds a launch and its sums' way through
 // memory.  Sides measured: 16384 x 1280 x 1280 256-tiles 47 us, 128-tiles 41; 4096^3 57 and 73; 512 x 8192 x 8192 128-tiles
 // 46, 64-tiles 59; 1024 x 1280 x 1280 12.1 and 11.2; 128 x 8192 x 8192 64-tiles whole 28.6, K cut in two 25.5.
-static Plan plan_of(int64_t M, int64_t N, int kb, bool exact) {
+static Plan plan_of(int64_t M, int64_t N, int kb, bool exact, bool whole_k = false) {
   struct Kind {
     int size, resident;
     double step;
@@ -616,7 +641,7 @@ static Plan plan_of(int64_t M, int64_t N, int kb, bool exact) {
     const double edge = 32.0 * t.size, slots = 256.0 * t.resident;
     const double whole = (double)((M + 32 * t.size - 1) / (32 * t.size)) * (double)((N + 32 * t.size - 1) / (32 * t.size));
     for (int parts = 1; parts <= 16; parts *= 2) {
-      if (parts > 1 && (kb < 4 * parts || whole * parts > 1024)) break;
+      if (parts > 1 && (whole_k || kb < 4 * parts || whole * parts > 1024)) break;
       const double work = whole * parts, steps = (double)((kb + parts - 1) / parts);
       auto round = [&](double n) {
         if (n <= 0) return 0.0;
@@ -635,10 +660,10 @@ static Plan plan_of(int64_t M, int64_t N, int kb, bool exact) {
   return best;
 }
 
-template <int WTM, int WTN, int S, int OUT_DT, bool EXACT>
+template <int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS = false>
 static hipError_t launch_tile(const Fp8Gemm& g, int parts, hipStream_t stream) {
   const int tiles_m = (int)((g.M + 32 * WTM - 1) / (32 * WTM)), tiles_n = (int)((g.N + 32 * WTN - 1) / (32 * WTN));
-  hipLaunchKernelGGL((tile_kernel<WTM, WTN, S, OUT_DT, EXACT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), 0, stream, g,
+  hipLaunchKernelGGL((tile_kernel<WTM, WTN, S, OUT_DT, EXACT, TAPS>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), 0, stream, g,
                      tiles_m, tiles_n);
   return hipGetLastError();
 }
@@ -679,6 +704,18 @@ static hipError_t launch_gemm(const Fp8Gemm& g, void* partial, hipStream_t strea
   hipLaunchKernelGGL((join_kernel<OUT_DT>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, (const float*)partial,
                      p.parts, g.bias, g.out, (long)g.M, (long)g.N);
   return hipGetLastError();
+}
+
+hipError_t launch_fp8_gemm(const Fp8Gemm& g, hipStream_t stream) {
+  const Plan p = plan_of(g.M, g.N, g.kb * g.ntaps, false, true);
+  if (g.ntaps > 1) {
+    if (g.out_dt != DT_BF16 || g.resid) return hipErrorInvalidValue;
+    if (p.size == 8) return launch_tile<8, 8, 2, DT_BF16, false, true>(g, 1, stream);
+    if (p.size == 4) return launch_tile<4, 4, 2, DT_BF16, false, true>(g, 1, stream);
+    return launch_tile<2, 2, 4, DT_BF16, false, true>(g, 1, stream);
+  }
+  if (g.out_dt == DT_BF16) return g.resid ? hipErrorInvalidValue : launch_plan<DT_BF16, false>(g, p, stream);
+  return g.out_dt == DT_FP32 ? launch_plan<DT_FP32, false>(g, p, stream) : hipErrorInvalidValue;
 }
 
 // workspace: the quantised rows (a multiple of 128 bytes), their scales, (kb, rows), up to 16 bytes, then the parts of a cut K loop

@@ -1,0 +1,34 @@
+// Blocks of 128 values in 8 bits (OCP e4m3) with a power-of-two scale: what the kernels that write them share.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace ed {
+
+// E8M0 byte of the scale for a block whose largest magnitude has these bits: 448 = 2^8 * (1 + 0x600000 / 2^23).
+__device__ __forceinline__ int scale_byte(unsigned amax) {
+  const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e < 1 ? 1 : e > 254 ? 254 : e;
+}
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }  // 2^(127 - byte)
+
+// largest magnitude (as bits) of eight values; Inf and NaN do not count and become NaN
+__device__ __forceinline__ unsigned amax8(float (&v)[8]) {
+  unsigned a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
+    if (b >= 0x7f800000u) v[i] = __builtin_nanf("");
+    else a = b > a ? b : a;
+  }
+  return a;
+}
+__device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
+  uint2 r;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+  r.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
+  r.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, w, true);
+  return r;
+}
+
+}  // namespace ed

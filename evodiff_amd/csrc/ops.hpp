@@ -16,8 +16,13 @@ inline int64_t fp8_blocks(int64_t k) { return (k + FP8_BLOCK - 1) / FP8_BLOCK; }
 hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, int64_t rows, int64_t K, uint8_t* q,
                                     uint8_t* scale, hipStream_t stream);
 // w (N, K) -> q (N, Kb * 128) and scale (ceil(N / 128), Kb): one scale for 128 x 128 weights
+// (kb_row > 0: into rows of kb_row blocks, from block b_first on - the taps of a convolution side by side)
 hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride, int64_t N, int64_t K, uint8_t* q,
-                                      uint8_t* scale, hipStream_t stream);
+                                      uint8_t* scale, hipStream_t stream, int kb_row = 0, int b_first = 0);
+// q, scale (kb, q_rows) <- act(LayerNorm(in)) in 8 bits: row r of `in` (fp32 or bf16, C channels) goes to row
+// (r / L) * seq_pitch + row0 + r % L.  act: 0 none, 1 GELU (the bf16 path's fit), 2 ReLU.
+hipError_t launch_ln_act_fp8(const void* in, bool in_bf16, const float* gamma, const float* beta, int rows, int C, int act, uint8_t* q,
+                             uint8_t* scale, long q_rows, int L, long seq_pitch, long row0, hipStream_t stream);
 
 // out[m][n] = bias[n] + sum_b 2^(xs[b][m] + ws[n / 128][b] - 254) sum_{k in block b} xq[m][k] * wq[n][k]
 struct Fp8Gemm {
@@ -27,8 +32,16 @@ struct Fp8Gemm {
   void* out;               // (M, N) of type out_dt
   int out_dt;
   int64_t M, N;
-  int kb;                  // blocks along K
+  int kb;                  // blocks along K (of one tap)
+  const float* resid = nullptr;  // fp32 (M, N) added to an fp32 result (may be out)
+  // A dilated convolution (ntaps > 1): output row m = (sequence, l) = (m / L, m % L) reads rows sequence * x_seq_pitch + x_row0 + l +
+  // (tap - center) * dilation of the x_rows rows of x, and weight rows hold ntaps * kb blocks, tap by tap.
+  int ntaps = 1, dilation = 1, center = 0, L = 1;
+  long x_seq_pitch = 0, x_row0 = 0, x_rows = 0;
 };
+// Without a workspace (K whole): bf16 results, fp32 results with or without a residual (rounded as the 8-bit instruction does),
+// bf16 results of a convolution.
+hipError_t launch_fp8_gemm(const Fp8Gemm& g, hipStream_t stream);
 
 // The product on plain or quantised rows (x_dt DT_E4M3: x_scale is read, row_stride is Kb * 128).
 enum { DT_E4M3 = 3 };  // = ED_DT_E4M3

@@ -109,14 +109,16 @@ class ByteNetTime(_ParamOnly):
         self.dropout = dropout
 
 
-_PRECISIONS = {"fp32": _lib.PREC_FP32, "bf16": _lib.PREC_BF16}
+_PRECISIONS = {"fp32": _lib.PREC_FP32, "bf16": _lib.PREC_BF16, "fp8": _lib.PREC_FP8}
 
 
 class ByteNetLMTime(nn.Module):
     """Drop-in for ``evodiff.model.ByteNetLMTime`` whose forward and samplers run in libevodiff_hip.so.
 
     ``precision``: "bf16" (fast path: bf16 MFMA operands, fp32 accumulate/residual/LayerNorm) or "fp32"
-    (validation path, fp32 MFMA).  Default from ``$EVODIFF_AMD_PRECISION`` or "bf16".
+    (validation path, fp32 MFMA).  Default from ``$EVODIFF_AMD_PRECISION`` or "bf16".  "fp8" (8-bit operands with a
+    power-of-two scale for each block of 128, fp32 accumulate/residual/LayerNorm) runs the forward and the scoring calls; the
+    fused sampling loops refuse it.
     """
 
     def __init__(self, n_tokens, d_embedding, d_model, n_layers, kernel_size, r, rank=None, n_frozen_embs=None,
@@ -190,7 +192,7 @@ class ByteNetLMTime(nn.Module):
         try:
             return _PRECISIONS[self.precision]
         except KeyError:
-            raise ValueError("precision must be 'fp32' or 'bf16', got %r" % (self.precision,))
+            raise ValueError("precision must be 'fp32', 'bf16' or 'fp8', got %r" % (self.precision,))
 
     # ------------------------------------------------------------------ reference call surface
     def _check_ranges(self, x, y, targets=None, select=None, n_classes=None):

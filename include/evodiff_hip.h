@@ -42,7 +42,10 @@ enum {
   ED_ENOMEM = -4
 };
 
-enum { ED_PREC_FP32 = 0, ED_PREC_BF16 = 1 };
+/* ED_PREC_FP8 (ed_forward, ed_forward_collect, ed_score_nll, ed_score_tokens): every product of the block stack takes both
+ * operands in the block-scaled 8-bit form described at ed_fp8_quantize_rows (weights are laid out at the first such call, which
+ * synchronises once); LayerNorms, the residual stream and all sums stay fp32, the vocabulary projection fp32. */
+enum { ED_PREC_FP32 = 0, ED_PREC_BF16 = 1, ED_PREC_FP8 = 2 };
 
 /* Hyper-parameters of ByteNetLMTime as constructed by evodiff/pretrained.py:39-42 from
  * config/config{38M,640M}.json (n_tokens=31, final_ln=True, tie_weights=False, causal=False). */
