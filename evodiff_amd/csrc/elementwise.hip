@@ -423,23 +423,19 @@ __global__ __launch_bounds__(256) void ln_act_fp8_kernel(const void* __restrict_
   for (int c = 0; c < NC8; ++c) {
     const int k = c * 512 + lane * 8, blk = k >> 7;
     if (blk >= kb) continue;  // (whole groups of 16 lanes)
-    float y[8];
+    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k < C) {
+      const float4 g0 = *(const float4*)(gamma + k), g1 = *(const float4*)(gamma + k + 4);
+      const float4 b0 = *(const float4*)(beta + k), b1 = *(const float4*)(beta + k + 4);
+      const float gm[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w}, bt[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float t = 0.f;
-      if (k < C) {
-        t = fmaf(v[c][j] * rstd, gamma[k + j], beta[k + j]);
-        if constexpr (ACT == 1) t = gelu_sigmoid_fit(t);
-        else if constexpr (ACT == 2) t = fmaxf(t, 0.f);
+      for (int j = 0; j < 8; ++j) {
+        y[j] = fmaf(v[c][j] * rstd, gm[j], bt[j]);
+        if constexpr (ACT == 1) y[j] = gelu_sigmoid_fit(y[j]);
+        else if constexpr (ACT == 2) y[j] = fmaxf(y[j], 0.f);
       }
-      y[j] = t;
     }
-    unsigned a = amax8(y);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      const unsigned b = (unsigned)__shfl_xor((int)a, o);
-      a = b > a ? b : a;
-    }
+    const unsigned a = max16(amax8(y));
     const int byte = scale_byte(a);
     *(uint2*)(q + (orow * kb + blk) * 128 + (k & 127)) = pack8(y, inverse_scale(byte));
     if ((lane & 15) == 0) scale[(long)blk * q_rows + orow] = (uint8_t)byte;

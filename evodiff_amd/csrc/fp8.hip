@@ -59,12 +59,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
   for (int u = 0; u < U; ++u) {
     const int b = b0 + u;
     if (b >= kb) break;
-    unsigned a = amax8(v[u]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      const unsigned c = (unsigned)__shfl_xor((int)a, o);
-      a = c > a ? c : a;
-    }
+    const unsigned a = max16(amax8(v[u]));
     const int byte = scale_byte(a);
     *(uint2*)(q + (row * kb + b) * FP8_BLOCK + l * 8) = pack8(v[u], inverse_scale(byte));
     if (l == 0) scale[TURNED ? b * rows + row : row * kb + b] = (uint8_t)byte;
@@ -401,9 +396,15 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
       T_out* const to = out + m * g.N + n;
       if constexpr (OUT_DT == DT_FP32 && !EXACT)
         if (g.resid) {  // (may be the output: a lane reads what it writes)
+          const float* const from = g.resid + m * g.N + n;
+          if (wide && n + 8 <= g.N) {
+            acc[2 * J][i] += *(const f32x4*)from;
+            acc[2 * J + 1][i] += *(const f32x4*)(from + 4);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < g.N) acc[2 * J + (e >> 2)][i][e & 3] += g.resid[m * g.N + n + e];
+            for (int e = 0; e < 8; ++e)
+              if (n + e < g.N) acc[2 * J + (e >> 2)][i][e & 3] += from[e];
+          }
         }
       if (wide && n + 8 <= g.N) {
         V8 v;

@@ -31,4 +31,13 @@ __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
   return r;
 }
 
+// largest of 16 neighbouring lanes (a row of the data-parallel moves), in every one of them
+__device__ __forceinline__ unsigned max16(unsigned a) {
+  auto step = [](unsigned v, unsigned o) { return o > v ? o : v; };
+  a = step(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xf, 0xf, true));   // quad_perm [1,0,3,2]
+  a = step(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E, 0xf, 0xf, true));   // quad_perm [2,3,0,1]
+  a = step(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x141, 0xf, 0xf, true));  // row_half_mirror
+  return step(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x140, 0xf, 0xf, true));  // row_mirror
+}
+
 }  // namespace ed
