@@ -148,7 +148,7 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Tiled product.  Four waves, 2 (rows) x 2 (channels), own a tile of 32 WTM rows x 32 WTN channels, a wave 16 WTM x 16 WTN as
+// Tiled product.  WM x 2 waves (rows x channels) own a tile of 16 WM WTM rows x 32 WTN channels, a wave 16 WTM x 16 WTN as
 // WTN x WTM instructions of 16 x 16 x 128: one per block of K and pair of fragments, its scales beside it.
 //
 // Step of K (one block): rows of 128 bytes of both operands, copied memory -> LDS into a ring of S stages, S - 1 steps ahead.
@@ -171,12 +171,17 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 // TAPS: the rows are positions of sequences and every one is multiplied from `ntaps` of them (a dilated convolution): K runs over
 // taps, then blocks; a tap moves the row operand by `dilation` rows of its padded layout, whose rows around a sequence hold
 // zeros.  Taps that move a whole tile outside its sequence are left out.
-template <int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS>
-__global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
-  constexpr int BM = 32 * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
-  constexpr int GX = BM / 32, GW = BN / 32, NG = GX + GW;  // 8-row copies a wave makes of each operand
+template <int WM, int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS>
+__global__ __launch_bounds__(128 * WM, WM / 2) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
+  constexpr int WAVES = 2 * WM, BM = 16 * WM * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
+  constexpr int GX = BM / 8 / WAVES, GW = BN / 8 / WAVES, NG = GX + GW;  // 8-row copies a wave makes of each operand
+  static_assert(GX * 8 * WAVES == BM && GW * 8 * WAVES == BN, "the copies cover the tile");
   constexpr int RING = 4, JB = WTN > 4 ? WTN - 3 : WTN > 2 ? WTN - 2 : 1;  // the barrier stands before row JB of instructions
   static_assert(JB >= WTN - RING + 1 && JB >= 1, "every channel fragment of a step is read in front of its barrier");
+  // the next step's channel fragment f (0 or 1) is read once no row of instructions needs its slot: from this row on (WTN: behind the last)
+  constexpr int FREE0 = (WTN - 1) / RING * RING + 1, FREE1 = (WTN - 2) / RING * RING + 2;
+  constexpr int W0_AT = FREE0 > JB ? FREE0 : JB, W1_AT = FREE1 > JB ? FREE1 : JB;
+  constexpr int NSW = 16 * WTN > 128 ? 2 : 1;  // blocks of channels that a wave's lie in
   static_assert((S & (S - 1)) == 0 && S >= 2, "the ring index is masked");
   __shared__ __attribute__((aligned(1024))) char lds[S * STAGE];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -231,23 +236,38 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
     const int ch = (lr & ~31) + 8 * ((lr & 15) >> 2) + 4 * ((lr >> 4) & 1) + (lr & 3);
     off[GX + j] = (unsigned)(ch * w_pitch) + ((wid * GW + j) & 1 ? chunk1 : chunk0);
   }
-  const long x_rows = TAPS ? g.x_rows : g.M;
-  const buffer_t x_src = buffer_of(g.xq + x_first * x_pitch, (x_rows - x_first) * x_pitch);
-  const buffer_t w_src = buffer_of(g.wq + n0 * w_pitch, (g.N - n0) * w_pitch);
-  // Past the last step the copies repeat its block (in bounds, into a stage nobody reads).
+  // Where the copies stand, bytes into a row of each operand; past the last step they repeat its block (in bounds, into a
+  // stage nobody reads).  The scales are read a step ahead and stand at their own place.
   const int last = T - 1;
-  auto copy = [&](int j, int t, char* stage) {  // piece j of step t
-    const unsigned b = (unsigned)(first + (t < last ? t : last));
-    if (j < GX) {
-      const unsigned tap = TAPS ? b / (unsigned)g.kb : 0;
-      const unsigned at = TAPS ? tap * (unsigned)g.dilation * (unsigned)x_pitch + (b - tap * (unsigned)g.kb) * FP8_BLOCK : b * FP8_BLOCK;
-      copy16(x_src, off[j], at, stage + (wid * GX + j) * 1024);
+  const unsigned first_tap = TAPS ? (unsigned)first / (unsigned)g.kb : 0, first_k = (unsigned)first - first_tap * (unsigned)g.kb;
+  struct Place {
+    unsigned x, w;  // of the row operand, of the weights
+    int k, t;       // block of the tap, step
+  };
+  Place at{first_tap * (unsigned)(TAPS ? g.dilation : 0) * (unsigned)x_pitch + first_k * FP8_BLOCK, (unsigned)first * FP8_BLOCK, (int)first_k, 0};
+  const unsigned x_rows = (unsigned)(TAPS ? g.x_rows : g.M);
+  Place sc{first_k * x_rows + first_tap * (unsigned)(TAPS ? g.dilation : 0), (unsigned)first, (int)first_k, 0};
+  auto advance = [&](Place& p, unsigned x_block, unsigned x_tap, unsigned w_block) {
+    if (p.t >= last) return;
+    ++p.t;
+    p.w += w_block;
+    if (TAPS && ++p.k == g.kb) {
+      p.k = 0;
+      p.x += x_tap - (unsigned)(g.kb - 1) * x_block;
     } else {
-      copy16(w_src, off[j], b * FP8_BLOCK, stage + BM * 128 + (wid * GW + j - GX) * 1024);
+      p.x += x_block;
     }
   };
+  auto advance_copies = [&]() { advance(at, FP8_BLOCK, TAPS ? (unsigned)g.dilation * (unsigned)x_pitch : 0, FP8_BLOCK); };
+  auto advance_scales = [&]() { advance(sc, x_rows, TAPS ? (unsigned)g.dilation : 0, 1); };
+  const buffer_t x_src = buffer_of(g.xq + x_first * x_pitch, ((long)x_rows - x_first) * x_pitch);
+  const buffer_t w_src = buffer_of(g.wq + n0 * w_pitch, (g.N - n0) * w_pitch);
+  auto copy = [&](int j, char* stage) {  // piece j of the step the copies stand at
+    if (j < GX) copy16(x_src, off[j], at.x, stage + (wid * GX + j) * 1024);
+    else copy16(w_src, off[j], at.w, stage + BM * 128 + (wid * GW + j - GX) * 1024);
+  };
 
-  // scales: a lane's row in each of the WTM fragments; the wave's channels lie in one block of 128
+  // scales: a lane's row in each of the WTM fragments; the wave's channels lie in NSW blocks of 128
   unsigned sx_row[TAPS ? WTM : 1];
   if constexpr (TAPS)
 #pragma unroll
@@ -258,13 +278,12 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   else
     sx_row[0] = (unsigned)(m0 + wr * 16 * WTM + fr);
   const long nw = n0 + wc * 16 * WTN;
-  const buffer_t sx_src = buffer_of(g.xs, x_rows * (long)g.kb);  // (kb, rows)
-  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * kb_all, kb_all);
-  auto row_scale = [&](int i, unsigned b) {  // of fragment i at block b
-    const unsigned tap = TAPS ? b / (unsigned)g.kb : 0;
-    const unsigned at = TAPS ? (b - tap * (unsigned)g.kb) * (unsigned)x_rows + tap * (unsigned)g.dilation : b * (unsigned)x_rows;
-    return load_byte(sx_src, TAPS ? sx_row[TAPS ? i : 0] : sx_row[0] + i * 16, at);
-  };
+  const buffer_t sx_src = buffer_of(g.xs, (long)x_rows * g.kb);  // (kb, rows)
+  // (past the last channel the byte reads as zero, or is another block's: those channels are not stored)
+  const buffer_t sw_src = buffer_of(g.ws + ((nw < g.N ? nw : g.N - 1) >> 7) * kb_all, ((g.N + 127) / 128 - ((nw < g.N ? nw : g.N - 1) >> 7)) * kb_all);
+  const int in_first = (int)(128 - (nw & 127)) >> 5;  // 32-channel pairs of fragments in the first of two blocks
+  auto row_scale = [&](int i) { return load_byte(sx_src, TAPS ? sx_row[TAPS ? i : 0] : sx_row[0] + i * 16, sc.x); };  // of fragment i
+  auto channel_scale_byte = [&](int k) { return load_byte(sw_src, 0, sc.w + (unsigned)(k * kb_all)); };
 
   const int swz = (fq ^ ((fr >> 1) & 7)) << 4;
   const int x_rd = (wr * 16 * WTM + fr) * 128, w_rd = BM * 128 + (wc * 16 * WTN + fr) * 128;
@@ -279,19 +298,23 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   bf16x8 XW[EXACT ? WTM : 1][4], WW[4];
   f32x4 part[2];
   int sx_now[WTM];
-  int sx[WTM], sx_next[WTM], sw, sw_next;
+  int sx[WTM], sx_next[WTM], sw[NSW], sw_next[NSW];
+  auto channel_scale = [&](int j) { return NSW == 1 || (j >> 1) < in_first ? sw[0] : sw[NSW - 1]; };
 
   // step 0 and its first fragments, copies of the S - 1 steps behind it
 #pragma unroll
-  for (int j = 0; j < NG; ++j) copy(j, 0, lds);
+  for (int j = 0; j < NG; ++j) copy(j, lds);
 #pragma unroll
-  for (int i = 0; i < WTM; ++i) sx[i] = row_scale(i, (unsigned)first);
-  sw = load_byte(sw_src, 0, (unsigned)first);
+  for (int i = 0; i < WTM; ++i) sx[i] = row_scale(i);
+#pragma unroll
+  for (int k = 0; k < NSW; ++k) sw[k] = channel_scale_byte(k);
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-  for (int k = 1; k < S; ++k)
+  for (int k = 1; k < S; ++k) {
+    advance_copies();
 #pragma unroll
-    for (int j = 0; j < NG; ++j) copy(j, k, lds + k * STAGE);
+    for (int j = 0; j < NG; ++j) copy(j, lds + k * STAGE);
+  }
 #pragma unroll
   for (int i = 0; i < WTM; ++i) { put(X[i], 0, read(lds, x_rd + i * 2048, 0)); put(X[i], 1, read(lds, x_rd + i * 2048, 1)); }
 #pragma unroll
@@ -300,7 +323,8 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
   for (int t = 0; t < T; ++t) {
     char* const here = lds + (t & (S - 1)) * STAGE;
     const char* const there = lds + ((t + 1) & (S - 1)) * STAGE;
-    const unsigned next = (unsigned)(first + (t < last ? t + 1 : last));
+    advance_copies();
+    advance_scales();
     if constexpr (EXACT)
 #pragma unroll
       for (int i = 0; i < WTM; ++i) sx_now[i] = sx[i];  // (sx becomes the next step's during the last row of instructions)
@@ -310,7 +334,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
         // Behind the copies of step t + 1 at least those of S - 2 steps and this step's scale loads were issued: with no more
         // than that many outstanding they have landed.  This wave's reads of the stage are in registers.
         __builtin_amdgcn_sched_barrier(0);
-        constexpr int OUT = (S - 2) * NG + WTM + 1;
+        constexpr int OUT = (S - 2) * NG + WTM + NSW;
         static_assert(OUT < 64, "the counter has six bits");
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
         __builtin_amdgcn_sched_barrier(0);
@@ -331,10 +355,10 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
           for (int h = 0; h < 4; ++h) now = __builtin_amdgcn_mfma_f32_16x16x32_bf16(WW[h], XW[i][h], now, 0, 0, 0);
           if (j * WTM + i > 0) {
             const int before = j * WTM + i - 1;
-            add_scaled(acc[before / WTM][before % WTM], part[before & 1], sx_now[before % WTM], sw);
+            add_scaled(acc[before / WTM][before % WTM], part[before & 1], sx_now[before % WTM], channel_scale(before / WTM));
           }
         } else {
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, sw, 0, sx[i]);
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[j % RING], X[i], acc[j][i], 0, 0, 0, channel_scale(j), 0, sx[i]);
         }
         const int slot = j * WTM + i;
         if (j < JB) {
@@ -345,22 +369,23 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
             if (want == slot) put(W[f % RING], r & 1, read(here, w_rd + f * 2048, r & 1));
           }
           constexpr int AT = JB * WTM >= 4 + WTM ? 4 : 0;  // the next step's scales
-          if (slot >= AT && slot < AT + WTM) sx_next[slot - AT] = row_scale(slot - AT, next);
-          if (slot == AT) sw_next = load_byte(sw_src, 0, next);
+          if (slot >= AT && slot < AT + WTM) sx_next[slot - AT] = row_scale(slot - AT);
+          if (slot == AT)
+#pragma unroll
+            for (int k = 0; k < NSW; ++k) sw_next[k] = channel_scale_byte(k);
         } else {
           constexpr int COPY_SLOTS = (WTN - JB) * WTM;
           const int after = slot - JB * WTM;
 #pragma unroll
-          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, t + S, here);
-          // the next step's first two channel fragments: slot 0 is free, slot 1 too unless row JB of instructions reads it
-          constexpr int W1_AT = JB % RING == 1 ? WTM : 2;
-          if (after < 2) put(W[0], after, read(there, w_rd, after));
-          if (after >= W1_AT && after < W1_AT + 2) put(W[1], after - W1_AT, read(there, w_rd + 2048, after - W1_AT));
+          for (int c = after * NG / COPY_SLOTS; c < (after + 1) * NG / COPY_SLOTS; ++c) copy(c, here);
+          const int from0 = slot - W0_AT * WTM, from1 = slot - W1_AT * WTM - (W1_AT == W0_AT ? 2 : 0);
+          if (from0 == 0 || from0 == 1) put(W[0], from0, read(there, w_rd, from0));
+          if (from1 == 0 || from1 == 1) put(W[1], from1, read(there, w_rd + 2048, from1));
           if (j == WTN - 1) {
             put(X[i], 0, read(there, x_rd + i * 2048, 0));  // in place: X[i] has done its last instruction of the step
             put(X[i], 1, read(there, x_rd + i * 2048, 1));
             sx[i] = sx_next[i];
-            if (W1_AT >= COPY_SLOTS && i == WTM - 1) {
+            if (W1_AT == WTN && i == WTM - 1) {
               put(W[1], 0, read(there, w_rd + 2048, 0));
               put(W[1], 1, read(there, w_rd + 2048, 1));
             }
@@ -369,8 +394,9 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(Fp8Gemm g, int tiles_m, in
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if constexpr (EXACT) add_scaled(acc[WTN - 1][WTM - 1], part[(WTN * WTM - 1) & 1], sx_now[WTM - 1], sw);
-    sw = sw_next;
+    if constexpr (EXACT) add_scaled(acc[WTN - 1][WTM - 1], part[(WTN * WTM - 1) & 1], sx_now[WTM - 1], channel_scale(WTN - 1));
+#pragma unroll
+    for (int k = 0; k < NSW; ++k) sw[k] = sw_next[k];
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no copy may land once this workgroup's shared memory is another's)
 
@@ -619,35 +645,36 @@ hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride,
   return hipGetLastError();
 }
 
-// How a product is cut: tiles of 32 `size` x 32 `size`, and the pieces of its K loop.
+// How a product is cut: tiles of 32 `size` x 32 `size` (10: 256 x 320), and the pieces of its K loop.
 struct Plan {
   int size, parts;
 };
 // The cheapest by what was measured of the tiles (microseconds).  A step of K takes a tile no less than `step` alone on its CU (its
 // latency), all tiles at work together no less than their copies take at 16 GB/ms of L2 and their products at `rate`; a round of
 // tiles has 2 to 3 us of start and end, and its results to write.  A cut K loop adds a launch and its sums' way through
-// memory.  Sides measured: 16384 x 1280 x 1280 256-tiles 47 us, 128-tiles 41; 4096^3 57 and 73; 512 x 8192 x 8192 128-tiles
+// memory.  Sides measured: 16384 x 1280 x 1280 tiles of 256 x 320 34 us, 256 x 256 47, 128 x 128 41; 4096^3 67, 55 and 69; 512 x 8192 x 8192 128-tiles
 // 46, 64-tiles 59; 1024 x 1280 x 1280 12.1 and 11.2; 128 x 8192 x 8192 64-tiles whole 28.6, K cut in two 25.5.
 static Plan plan_of(int64_t M, int64_t N, int kb, bool exact, bool whole_k = false) {
   struct Kind {
-    int size, resident;
+    int size, bm, bn, resident;
     double step;
   };
-  static const Kind fast[3] = {{8, 1, 1.1}, {4, 2, 0.6}, {2, 2, 0.24}}, wide[2] = {{4, 2, 1.55}, {2, 2, 0.75}};
+  static const Kind fast[4] = {{10, 256, 320, 1, 1.3}, {8, 256, 256, 1, 1.1}, {4, 128, 128, 2, 0.6}, {2, 64, 64, 2, 0.24}},
+                    wide[2] = {{4, 128, 128, 2, 1.55}, {2, 64, 64, 2, 0.75}};
   const double rate = exact ? 0.75e9 : 2.6e9, l2 = 16e6, hbm = 4.5e6;  // per microsecond
   Plan best{2, 1};
   double least = 1e30;
-  for (int k = 0; k < (exact ? 2 : 3); ++k) {
+  for (int k = 0; k < (exact ? 2 : 4); ++k) {
     const Kind& t = exact ? wide[k] : fast[k];
-    const double edge = 32.0 * t.size, slots = 256.0 * t.resident;
-    const double whole = (double)((M + 32 * t.size - 1) / (32 * t.size)) * (double)((N + 32 * t.size - 1) / (32 * t.size));
+    const double area = (double)t.bm * t.bn, slots = 256.0 * t.resident;
+    const double whole = (double)((M + t.bm - 1) / t.bm) * (double)((N + t.bn - 1) / t.bn);
     for (int parts = 1; parts <= 16; parts *= 2) {
       if (parts > 1 && (whole_k || kb < 4 * parts || whole * parts > 1024)) break;
       const double work = whole * parts, steps = (double)((kb + parts - 1) / parts);
       auto round = [&](double n) {
         if (n <= 0) return 0.0;
-        const double step = std::max({t.step, n * 2 * edge * 128 / l2, n * edge * edge * 256 / rate});
-        return steps * step + (t.resident > 1 ? 2.0 : 3.0) + n * edge * edge * (parts > 1 || exact ? 4 : 2) / hbm / t.resident;
+        const double step = std::max({t.step, n * (t.bm + t.bn) * 128 / l2, n * area * 256 / rate});
+        return steps * step + (t.resident > 1 ? 2.0 : 3.0) + n * area * (parts > 1 || exact ? 4 : 2) / hbm / t.resident;
       };
       const double full = std::floor(work / slots);
       double cost = full * round(slots) + round(work - full * slots);
@@ -661,21 +688,22 @@ static Plan plan_of(int64_t M, int64_t N, int kb, bool exact, bool whole_k = fal
   return best;
 }
 
-template <int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS = false>
+template <int WM, int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS = false>
 static hipError_t launch_tile(const Fp8Gemm& g, int parts, hipStream_t stream) {
-  const int tiles_m = (int)((g.M + 32 * WTM - 1) / (32 * WTM)), tiles_n = (int)((g.N + 32 * WTN - 1) / (32 * WTN));
-  hipLaunchKernelGGL((tile_kernel<WTM, WTN, S, OUT_DT, EXACT, TAPS>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), 0, stream, g,
-                     tiles_m, tiles_n);
+  const int tiles_m = (int)((g.M + 16 * WM * WTM - 1) / (16 * WM * WTM)), tiles_n = (int)((g.N + 32 * WTN - 1) / (32 * WTN));
+  hipLaunchKernelGGL((tile_kernel<WM, WTM, WTN, S, OUT_DT, EXACT, TAPS>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(128 * WM), 0,
+                     stream, g, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
 template <int OUT_DT, bool EXACT>
 static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t stream) {
   if constexpr (!EXACT) {
-    if (p.size == 8) return launch_tile<8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
+    if (p.size == 10) return launch_tile<4, 4, 10, 2, OUT_DT, EXACT>(g, p.parts, stream);
+    if (p.size == 8) return launch_tile<2, 8, 8, 2, OUT_DT, EXACT>(g, p.parts, stream);
   }
-  if (p.size == 4) return launch_tile<4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
-  return launch_tile<2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
+  if (p.size == 4) return launch_tile<2, 4, 4, 2, OUT_DT, EXACT>(g, p.parts, stream);
+  return launch_tile<2, 2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
 }
 
 constexpr int FEW_ROWS = 16;
@@ -711,9 +739,10 @@ hipError_t launch_fp8_gemm(const Fp8Gemm& g, hipStream_t stream) {
   const Plan p = plan_of(g.M, g.N, g.kb * g.ntaps, false, true);
   if (g.ntaps > 1) {
     if (g.out_dt != DT_BF16 || g.resid) return hipErrorInvalidValue;
-    if (p.size == 8) return launch_tile<8, 8, 2, DT_BF16, false, true>(g, 1, stream);
-    if (p.size == 4) return launch_tile<4, 4, 2, DT_BF16, false, true>(g, 1, stream);
-    return launch_tile<2, 2, 4, DT_BF16, false, true>(g, 1, stream);
+    if (p.size == 10) return launch_tile<4, 4, 10, 2, DT_BF16, false, true>(g, 1, stream);
+    if (p.size == 8) return launch_tile<2, 8, 8, 2, DT_BF16, false, true>(g, 1, stream);
+    if (p.size == 4) return launch_tile<2, 4, 4, 2, DT_BF16, false, true>(g, 1, stream);
+    return launch_tile<2, 2, 2, 4, DT_BF16, false, true>(g, 1, stream);
   }
   if (g.out_dt == DT_BF16) return g.resid ? hipErrorInvalidValue : launch_plan<DT_BF16, false>(g, p, stream);
   return g.out_dt == DT_FP32 ? launch_plan<DT_FP32, false>(g, p, stream) : hipErrorInvalidValue;

@@ -11,16 +11,20 @@ __device__ __forceinline__ int scale_byte(unsigned amax) {
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }  // 2^(127 - byte)
 
-// largest magnitude (as bits) of eight values; Inf and NaN do not count and become NaN
+// largest finite magnitude (as bits) of eight values; infinities become NaN (a NaN does not count by itself, and stays one)
 __device__ __forceinline__ unsigned amax8(float (&v)[8]) {
-  unsigned a = 0;
+  float a = fabsf(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
-    if (b >= 0x7f800000u) v[i] = __builtin_nanf("");
-    else a = b > a ? b : a;
+  for (int i = 1; i < 8; ++i) a = fmaxf(a, fabsf(v[i]));
+  if (a == __builtin_huge_valf()) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (fabsf(v[i]) == __builtin_huge_valf()) v[i] = __builtin_nanf("");
+      a = fmaxf(a, fabsf(v[i]));
+    }
   }
-  return a;
+  return a != a ? 0u : __float_as_uint(a);  // (all NaN: none)
 }
 __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv) {
   uint2 r;
