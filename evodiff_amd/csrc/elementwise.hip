@@ -364,6 +364,10 @@ __global__ __launch_bounds__(256) void ln_act_fast_kernel(const void* __restrict
   }
 }
 
+__global__ __launch_bounds__(256) void clear_kernel(uint4* __restrict__ p, long n) {
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) p[i] = uint4{0, 0, 0, 0};
+}
+
 // ---------------------------------------------------------------------------------------------------
 // LayerNorm + activation into blocks of 128 in 8 bits (ED_PREC_FP8): one pass, bound by HBM (a 1280-channel row in bf16 is 2.5 KB
 // in, 1.3 KB out).  A wave owns a row, 8 neighbouring channels a lane and chunk of 512, so that 16 lanes hold a block; the
@@ -431,8 +435,7 @@ __global__ __launch_bounds__(256) void ln_act_fp8_kernel(const void* __restrict_
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y[j] = fmaf(v[c][j] * rstd, gm[j], bt[j]);
-        if constexpr (ACT == 1) y[j] = gelu_sigmoid_fit(y[j]);
-        else if constexpr (ACT == 2) y[j] = fmaxf(y[j], 0.f);
+        y[j] = ACT == 1 ? gelu_sigmoid_fit(y[j]) : fmaxf(y[j], 0.f);
       }
     }
     const unsigned a = max16(amax8(y));
@@ -1019,17 +1022,23 @@ hipError_t launch_advance_step(StepState* state, hipStream_t stream) {
   return hipGetLastError();
 }
 
+hipError_t launch_clear(void* p, size_t bytes, hipStream_t stream) {
+  if (!p || bytes == 0 || bytes % 16) return hipErrorInvalidValue;
+  const size_t n = bytes / 16, blocks = (n + 255) / 256;
+  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (uint4*)p, (long)n);
+  return hipGetLastError();
+}
+
 hipError_t launch_ln_act_fp8(const void* in, bool in_bf16, const float* gamma, const float* beta, int rows, int C, int act, uint8_t* q,
                              uint8_t* scale, long q_rows, int L, long seq_pitch, long row0, hipStream_t stream) {
-  if (C % 8 || C > 2048 || rows < 1) return hipErrorInvalidValue;
+  if (C % 8 || C > 2048 || rows < 1 || (act != 1 && act != 2)) return hipErrorInvalidValue;
   const dim3 grid((rows + 3) / 4), block(256);
 #define ED_GO(NC8, BF, ACT)                                                                                               \
   hipLaunchKernelGGL((ln_act_fp8_kernel<NC8, BF, ACT>), grid, block, 0, stream, in, gamma, beta, rows, C, q, scale, q_rows, L, \
                      seq_pitch, row0)
 #define ED_ACT(NC8, BF)                                                                                                   \
   if (act == 1) ED_GO(NC8, BF, 1);                                                                                         \
-  else if (act == 2) ED_GO(NC8, BF, 2);                                                                                    \
-  else ED_GO(NC8, BF, 0)
+  else ED_GO(NC8, BF, 2)
 #define ED_CH(BF)                                                                                                         \
   if (C <= 512) { ED_ACT(1, BF); }                                                                                         \
   else if (C <= 1024) { ED_ACT(2, BF); }                                                                                   \

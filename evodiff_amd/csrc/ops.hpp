@@ -19,8 +19,10 @@ hipError_t launch_fp8_quantize_rows(const void* x, int dt, int64_t row_stride, i
 // (kb_row > 0: into rows of kb_row blocks, from block b_first on - the taps of a convolution side by side)
 hipError_t launch_fp8_quantize_weight(const void* w, int dt, int64_t row_stride, int64_t N, int64_t K, uint8_t* q,
                                       uint8_t* scale, hipStream_t stream, int kb_row = 0, int b_first = 0);
+// zeros, by a kernel (bytes: a multiple of 16)
+hipError_t launch_clear(void* p, size_t bytes, hipStream_t stream);
 // q, scale (kb, q_rows) <- act(LayerNorm(in)) in 8 bits: row r of `in` (fp32 or bf16, C channels) goes to row
-// (r / L) * seq_pitch + row0 + r % L.  act: 0 none, 1 GELU (the bf16 path's fit), 2 ReLU.
+// (r / L) * seq_pitch + row0 + r % L.  act: 1 GELU (the bf16 path's fit), 2 ReLU.
 hipError_t launch_ln_act_fp8(const void* in, bool in_bf16, const float* gamma, const float* beta, int rows, int C, int act, uint8_t* q,
                              uint8_t* scale, long q_rows, int L, long seq_pitch, long row0, hipStream_t stream);
 

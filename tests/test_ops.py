@@ -696,3 +696,133 @@ def test_model_score_tokens(dev):
         m.score_tokens(x, y, targets[:, :-1])
     with pytest.raises(_lib.EvoDiffHipError):
         m.score_tokens(x, y, torch.full_like(targets, 30), n_classes=26)
+
+
+# ---- the model in 8 bits --------------------------------------------------------------------------------------------
+
+def bytenet(d_model, n_layers, r, slim=True, activation="gelu", causal=False, timesteps=None, kernel_size=5):
+    from evodiff_amd.model import ByteNetLMTime
+    torch.manual_seed(3)
+    m = ByteNetLMTime(31, 8, d_model, n_layers, kernel_size, r, padding_idx=28, final_ln=True, slim=slim, activation=activation,
+                      causal=causal, timesteps=timesteps).eval()
+    with torch.no_grad():
+        for name, p in m.named_parameters():  # (norms and biases that are not their initial ones and zeros)
+            if p.dim() == 1:
+                p.add_(0.2 * torch.randn_like(p))
+    m.precision = "fp8"
+    return m
+
+
+def plain_block(block, dilation, x, causal, activation):
+    """What a block adds to the residual stream x (B, L, D), fp64 on the CPU: LayerNorms and activations in 64 bits, the operands
+    of each product rounded to 8 bits with the scales of the definition, products' outputs rounded to bf16 but the last."""
+    act = torch.nn.functional.gelu if activation == "gelu" else torch.relu
+
+    def rows(v, norm):
+        v = act(torch.nn.functional.layer_norm(v, v.shape[-1:], norm.weight.double().cpu(), norm.bias.double().cpu(), norm.eps))
+        flat = v.reshape(-1, v.shape[-1])
+        return dequantized(*plain_quantize(flat, False), False)[:, :v.shape[-1]].reshape(v.shape)
+
+    def weight(w):
+        return dequantized(*plain_quantize(w, True), True)[:, :w.shape[1]]
+
+    def bf16(v):
+        return v.bfloat16().double()
+
+    pff1, pff2, conv = block.sequence1[2].conv, block.sequence2[2].conv, block.conv
+    y = bf16(rows(x, block.sequence1[0]) @ weight(pff1.weight[:, :, 0]).T + pff1.bias.double())
+    z = rows(y, block.sequence1[3])
+    taps, length = conv.weight.shape[2], x.shape[1]
+    center = taps - 1 if causal else taps // 2
+    y = conv.bias.double().repeat(z.shape[0], length, 1)
+    for t in range(taps):
+        shift = (t - center) * dilation
+        lo, hi = max(0, -shift), min(length, length - shift)
+        if lo < hi:
+            y[:, lo:hi] += z[:, lo + shift:hi + shift] @ weight(conv.weight[:, :, t]).T
+    return rows(bf16(y), block.sequence2[0]) @ weight(pff2.weight[:, :, 0]).T + pff2.bias.double()
+
+
+@gpu
+@pytest.mark.parametrize("batch,length,kw", [
+    (3, 50, dict(d_model=256, n_layers=8, r=128)),                                       # taps that reach no row
+    (1, 1, dict(d_model=64, n_layers=2, r=2)),
+    (2, 300, dict(d_model=96, n_layers=3, r=4, slim=False, activation="relu")),          # channels that end inside a block
+    (5, 33, dict(d_model=320, n_layers=4, r=8, causal=True)),
+    (1, 129, dict(d_model=640, n_layers=2, r=2, timesteps=20, slim=False)),
+    (40, 64, dict(d_model=1024, n_layers=2, r=64)),
+    (7, 500, dict(d_model=384, n_layers=2, r=128, slim=False)),
+    (2, 70, dict(d_model=2048, n_layers=1, r=1, slim=False, kernel_size=3)),
+    (4, 100, dict(d_model=128, n_layers=2, r=2, kernel_size=1)),
+])
+def test_model_in_8_bits(dev, batch, length, kw):
+    """Every block against its plain form from the same residual stream, position by position, in 2-norms.
+
+    The first product's operands differ from the plain form's where a relative difference of 1e-6 in the LayerNorm (3e-5 with
+    the fitted GELU) turns a rounding: an expected square of difference * step, the steps 2^-4 to 2^-3 of a value, so 0.2 %; the
+    products keep that share, the second quantiser turns 2e-3 into sqrt(2e-3 * 0.09) = 1.3 %, the third that into 3.4 %.  The
+    bound is 10 %, three times that; a tap left out of five is 45 %, one of three blocks at twice its scale 58 %."""
+    m = bytenet(**kw)
+    x = torch.randint(0, 26, (batch, length), device=dev)
+    y = torch.randint(0, kw.get("timesteps") or 1, (batch,), device=dev)
+    logits, acts = m(x, y, return_blocks=True)
+    again = m(x, y)
+    assert torch.equal(logits, again)
+    acts = acts.double().cpu()
+    for i, (block, dilation) in enumerate(zip(m.embedder.layers, m.embedder.dilations)):
+        want = plain_block(block, dilation, acts[i], kw.get("causal", False), kw.get("activation", "gelu"))
+        got = acts[i + 1] - acts[i]
+        worst = float(((got - want).norm(dim=2) / want.norm(dim=2)).detach().max())
+        print("block", i, "dilation", dilation, "worst position", worst)
+        assert worst < 0.1
+    tail = torch.nn.functional.layer_norm(acts[-1], acts.shape[-1:], m.last_norm.weight.double(), m.last_norm.bias.double(), m.last_norm.eps)
+    tail = tail @ m.decoder.conv.weight[:, :, 0].double().T + m.decoder.conv.bias.double()
+    assert float((logits.cpu() - tail).abs().max()) < 1e-4 * float(tail.abs().max())
+
+
+@gpu
+def test_model_in_8_bits_scores_lengths_in_turn_and_new_weights(dev):
+    m = bytenet(256, 4, 8)
+    y = torch.zeros(6, dtype=torch.long, device=dev)
+    calls = [torch.randint(0, 26, s, device=dev) for s in ((6, 90), (2, 17), (5, 200), (6, 91), (1, 1))]
+    first = [m(x, y[:len(x)]) for x in calls]
+    for x, want in zip(reversed(calls), reversed(first)):  # the zero rows of one length are another's values
+        assert torch.equal(m(x, y[:len(x)]), want)
+    x, logits = calls[0], first[0]
+    targets = torch.randint(0, 26, x.shape, device=dev)
+    select = torch.rand(x.shape, device=dev) < 0.5
+    got = m.score_tokens(x, y, targets, select=select, n_classes=26, top_k=4)
+    want = plain_logprobs(logits.reshape(-1, 31), targets.reshape(-1).cpu(), 4, select.reshape(-1).cpu(), 26)
+    tol = logprob_tolerance(logits.cpu(), 26)
+    assert torch.equal(got.top_token.reshape(-1, 4).cpu(), want[3])
+    rel_ok(got.logprob.reshape(-1), want[0], tol)
+    rel_ok(got.entropy.reshape(-1), want[1], 2 * tol)
+    assert float((got.logprob + m.score_nll(x, y, targets, select=select, n_classes=26)).abs().max()) < 1e-4
+    with torch.no_grad():
+        m.embedder.layers[1].conv.weight.mul_(-1)
+    changed, acts = m(x, y, return_blocks=True)
+    assert not torch.equal(changed, logits)
+    acts = acts.double().cpu()
+    want = plain_block(m.embedder.layers[1], m.embedder.dilations[1], acts[1], False, "gelu")
+    assert float(((acts[2] - acts[1] - want).norm(dim=2) / want.norm(dim=2)).detach().max()) < 0.1
+    other = bytenet(256, 4, 8)
+    other.precision = "bf16"
+    other(x, y)
+    m.precision = "bf16"  # a handle that has run in 8 bits runs in the others as before
+    with torch.no_grad():
+        m.embedder.layers[1].conv.weight.mul_(-1)
+    m.precision = "fp8"
+    assert torch.equal(m(x, y), logits)
+    m.precision = "bf16"
+    assert torch.equal(m(x, y), other(x, y))
+
+
+@gpu
+def test_model_in_8_bits_refuses_the_sampling_loops(dev):
+    m = bytenet(64, 2, 2)
+    order = torch.arange(10, dtype=torch.int32, device=dev)
+    with pytest.raises(_lib.EvoDiffHipError, match="sampling loops"):
+        m.oadm_sample(torch.full((2, 10), 28, device=dev), order, torch.rand((10, 2), device=dev), 26)
+    m.precision = "fp4"
+    with pytest.raises(ValueError, match="fp8"):
+        m(torch.zeros((1, 4), dtype=torch.long, device=dev), torch.zeros(1, dtype=torch.long, device=dev))
