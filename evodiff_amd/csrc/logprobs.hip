@@ -681,8 +681,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
 
 // ---------------------------------------------------------------------------------------------------
 // Gradient: a value in, a value out.  log p comes from the row's saved maximum and log sum; the few classes that are named
-// (target, top alternatives) are written once more behind the rest of their tile by the workgroup that owns it, each as the
-// whole sum for its class, in a fixed order.
+// (target, top alternatives) get the whole sum for their class, in a fixed order.
 // ---------------------------------------------------------------------------------------------------
 struct GradRow {
   float m, log_s, h, weight, g_h;
@@ -692,8 +691,8 @@ struct GradRow {
     return -p * fmaf(g_h, max_nan(lp, -1.0e30f) + h, weight);  // (a forbidden class: nothing, not nothing times infinity)
   }
 };
-__device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* targets, const uint8_t* select, int top_k,
-                                            const LogprobsGrad& g, long r) {
+__device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* targets, const uint8_t* select,
+                                            const LogprobsGrad& g, long r) {  // (weight: without the top alternatives)
   GradRow a;
   a.m = g.stats[2 * r];
   a.log_s = g.stats[2 * r + 1];
@@ -701,8 +700,6 @@ __device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* 
   a.h = g.entropy[r];
   a.weight = g.g_logprob ? g.g_logprob[r] : 0.f;
   a.g_h = g.g_entropy ? g.g_entropy[r] : 0.f;
-  if (g.g_top)
-    for (int j = 0; j < top_k; ++j) a.weight += g.g_top[r * top_k + j];
   if (targets && (targets[r] < 0 || targets[r] >= x.n)) a.weight = __builtin_nanf("");
   return a;
 }
@@ -716,8 +713,10 @@ __device__ __forceinline__ float named(const int64_t* targets, int top_k, const 
 }
 
 // A workgroup per `per` tiles of 256 vectors of a row: 16-byte loads, the next tile's in flight, and 16-byte stores where source
-// and destination rows lie alike within 16 bytes; class by class elsewhere.  The named classes of the piece are listed in
-// shared memory while the first loads fly.
+// and destination rows lie alike within 16 bytes; class by class elsewhere.  The stores pass by the caches (the reader behind is a
+// product over the whole gradient): 4096 x 32000 bf16 117 -> 90 us, 1024 x 32000 fp32 56 -> 43.  The named classes of the piece are
+// listed in shared memory while the first loads fly, with a bit for each vector that holds one.
+constexpr int GRAD_TILES = 8;  // at most, of a workgroup
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const int64_t* __restrict__ targets,
                                                             const uint8_t* __restrict__ select, int top_k,
@@ -725,9 +724,12 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
   typedef typename Elem<DT>::T T;
   constexpr int EPV = 16 / sizeof(T), U = 2;
   typedef __attribute__((ext_vector_type(EPV))) T VT;
-  __shared__ int name_at[TOP_MAX + 1];
+  __shared__ int64_t cls[TOP_MAX + 1];  // named classes and their gradients, in order
+  __shared__ float cls_g[TOP_MAX + 1];
+  __shared__ int name_at[TOP_MAX + 1];  // those of this piece, each once, and their sums
   __shared__ float name_add[TOP_MAX + 1];
   __shared__ int n_names;
+  __shared__ unsigned hot[GRAD_TILES * 8];
   const int tid = threadIdx.x;
   const long items = x.rows * pieces;
   for (long item = blockIdx.x; item < items; item += gridDim.x) {
@@ -748,20 +750,35 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
         if (at + u * 256 + tid < v1) next[u] = *(const uint4*)(row + head + (long)(at + u * 256 + tid) * EPV);
     };
     load(v0);
-    const GradRow a = grad_row(x, targets, select, top_k, g, r);
-    __syncthreads();
-    if (tid == 0) n_names = 0;
-    __syncthreads();
+    GradRow a = grad_row(x, targets, select, g, r);
     const int has_target = g.g_logprob ? 1 : 0, names = has_target + (g.g_top ? top_k : 0);
+    __syncthreads();  // the row before is done with the shared memory
     if (tid < names) {
-      const int64_t v = has_target && tid == 0 ? targets[r] : g.top_token[r * top_k + tid - has_target];
-      if (v >= 0 && v < x.n) {
-        const int64_t vec = (v - head) / EPV;
-        const bool inside = v >= head && vec < vectors;
-        if (inside ? vec >= v0 && vec < v1 : true) {
-          const int slot = atomicAdd(&n_names, 1);  // (a class named twice is listed twice, with the same sum)
+      const bool target = has_target && tid == 0;
+      const long at = r * top_k + tid - has_target;
+      cls[tid] = target ? targets[r] : g.top_token[at];
+      cls_g[tid] = target ? g.g_logprob[r] : g.g_top[at];
+    }
+    if (tid == 0) n_names = 0;
+    if (tid < GRAD_TILES * 8) hot[tid] = 0;
+    __syncthreads();
+    for (int j = has_target; j < names; ++j) a.weight += cls_g[j];
+    if (tid < names) {
+      const int64_t v = cls[tid], vec = (v - head) / EPV;
+      const bool inside = v >= head && vec < vectors;
+      if (v >= 0 && v < x.n && (!inside || (vec >= v0 && vec < v1))) {
+        float d = 0.f;
+        bool first = true;
+        for (int j = 0; j < names; ++j)
+          if (cls[j] == v) {
+            first &= j >= tid;
+            d += cls_g[j];
+          }
+        if (first) {
+          const int slot = atomicAdd(&n_names, 1);
           name_at[slot] = (int)v;
-          name_add[slot] = named(targets, top_k, g, r, v);
+          name_add[slot] = d;
+          if (inside) atomicOr(&hot[(vec - v0) >> 5], 1u << ((vec - v0) & 31));
         }
       }
     }
@@ -781,21 +798,16 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
         unpack<DT>(raw[u], f);
 #pragma unroll
         for (int i = 0; i < EPV; ++i) f[i] = a.at(f[i]);
-        for (int j = 0; j < listed; ++j) {
-          const int off = name_at[j] - first;
-          if (off >= 0 && off < EPV) {
-            bool again = false;
-            for (int k = 0; k < j; ++k) again |= name_at[k] == name_at[j];
-            if (!again) {
+        if (hot[(vec - v0) >> 5] >> ((vec - v0) & 31) & 1)
+          for (int j = 0; j < listed; ++j) {
+            const int off = name_at[j] - first;
 #pragma unroll
-              for (int i = 0; i < EPV; ++i) f[i] += off == i ? name_add[j] : 0.f;
-            }
+            for (int i = 0; i < EPV; ++i) f[i] += off == i ? name_add[j] : 0.f;
           }
-        }
         VT o;
 #pragma unroll
         for (int i = 0; i < EPV; ++i) o[i] = Elem<DT>::put(a.skip ? 0.f : f[i]);
-        *(VT*)(dst + first) = o;
+        __builtin_nontemporal_store(o, (VT*)(dst + first));
       }
     }
     auto one = [&](long v) {
@@ -831,7 +843,9 @@ __global__ __launch_bounds__(256) void logprobs_grad_flat_kernel(LogitsView x, c
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
     const long r = i / g.columns;
     const int v = (int)(i - r * g.columns);
-    const GradRow a = grad_row(x, targets, select, top_k, g, r);
+    GradRow a = grad_row(x, targets, select, g, r);
+    if (g.g_top)
+      for (int j = 0; j < top_k; ++j) a.weight += g.g_top[r * top_k + j];
     float d = 0.f;
     if (!a.skip && v < x.n) d = a.at(Elem<DT>::get(row_of<T>(x, r)[v])) + named(targets, top_k, g, r, v);
     ((T*)g.dlogits)[i] = Elem<DT>::put(d);
@@ -911,7 +925,7 @@ static hipError_t launch_grad(const LogitsView& x, const int64_t* targets, const
     // tiles of 256 vectors in a workgroup: eight where the rows are many (the row's scalars and names are read once for
     // them), down to two so that few rows still fill the chip eight workgroups a CU deep
     const long tiles = (g.columns / (16 / dt_bytes(DT)) + 255) / 256;
-    int per = 8;
+    int per = GRAD_TILES;
     while (per > 2 && x.rows * ((tiles + per - 1) / per) < 2048) per /= 2;
     const int pieces = (int)((tiles + per - 1) / per);
     hipLaunchKernelGGL((logprobs_grad_kernel<DT>), blocks(x.rows * pieces), dim3(256), 0, stream, x, targets, select, top_k, g, pieces, per);
