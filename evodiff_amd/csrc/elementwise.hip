@@ -369,9 +369,11 @@ __global__ __launch_bounds__(256) void clear_kernel(uint4* __restrict__ p, long 
 }
 
 // ---------------------------------------------------------------------------------------------------
-// LayerNorm + activation into blocks of 128 in 8 bits (ED_PREC_FP8): one pass, bound by HBM (a 1280-channel row in bf16 is 2.5 KB
-// in, 1.3 KB out).  A wave owns a row, 8 neighbouring channels a lane and chunk of 512, so that 16 lanes hold a block; the
-// statistics are taken on the values in registers, mean first.
+// LayerNorm + activation into blocks of 128 in 8 bits (ED_PREC_FP8), one pass: a wave owns a row, 8 neighbouring channels a lane
+// and chunk of 512, so that 16 lanes hold a block; the statistics are taken on the values in registers, mean first.  16384 rows of
+// 1280 channels: 22 us from bf16 (63 MB, 13 us at the rate of a copy), 24 us from fp32 (105 MB, 22 us).  The bf16 form is bound by its
+// vector instructions, some 30 a value, eight of them the exponential and the reciprocal of the GELU: several rows a wave with
+// the next row's loads in flight and the affine parameters kept in registers took the same 22 us.
 // ---------------------------------------------------------------------------------------------------
 template <int NC8, bool IN_BF16, int ACT>
 __global__ __launch_bounds__(256) void ln_act_fp8_kernel(const void* __restrict__ in, const float* __restrict__ gamma,

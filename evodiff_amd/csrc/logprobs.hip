@@ -617,6 +617,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
                                                             const char* __restrict__ pieces, int splits) {
   typedef typename Elem<DT>::T T;
   __shared__ u64 keys[64 * TOP_MAX];
+  __shared__ alignas(16) u64 firsts[64 + TOP_MAX + 8];
   __shared__ alignas(16) u64 found[64 * TOP_MAX + 8];
   __shared__ u64 tau;
   __shared__ int n_found;
@@ -634,10 +635,16 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
       tau = 0;
       n_found = 0;
     }
+    const int64_t t = targets ? targets[r] : -1;  // (its value and the pieces are on their way together)
+    const float target_value = targets && t >= 0 && t < x.n ? Elem<DT>::get(row[t]) : 0.f;
+    const int depth = top_k ? (top_k + splits - 1) / splits : 0, n_firsts = depth * splits;  // < splits + top_k <= 96
     for (int i = tid; i < splits * top_k; i += 256) {
-      const int s = i / top_k;
-      keys[i] = ((const u64*)(src + s * piece_bytes(top_k) + sizeof(Piece)))[i - s * top_k];
+      const int s = i / top_k, j = i - s * top_k;
+      const u64 k = ((const u64*)(src + s * piece_bytes(top_k) + sizeof(Piece)))[j];
+      keys[i] = k;
+      if (j < depth) firsts[s * depth + j] = k;
     }
+    if (tid < 8) firsts[n_firsts + tid] = 0;
     Sums2 a{NEG_INF, R_MIN, 0.f, 0.f};  // every wave joins all pieces, one a lane
     if ((tid & 63) < splits) a = ((const Piece*)(src + (tid & 63) * piece_bytes(top_k)))->sums;
 #pragma unroll
@@ -648,20 +655,22 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitsView x, const 
     const bool plain = (a.m > PLAIN_FROM || a.m < -PLAIN_FROM) && a.m != NEG_INF;
     const RowEnd res = plain ? RowEnd(plain_sums<DT, 256>(row, x.n, plain_space, tid)) : RowEnd(a);
     if (tid == 0) {
-      if (targets) {
-        const int64_t t = targets[r];
-        out.logprob[r] = t < 0 || t >= x.n ? __builtin_nanf("") : res.logprob(Elem<DT>::get(row[t]));
-      }
+      if (targets) out.logprob[r] = t < 0 || t >= x.n ? __builtin_nanf("") : res.logprob(target_value);
       out.entropy[r] = res.entropy;
       if (out.stats) put_stats(out.stats + 2 * r, res.mark(), res.log_s);
     }
     if (top_k == 0) continue;
     __syncthreads();
-    const int depth = (top_k + splits - 1) / splits, firsts = depth * splits;  // firsts < splits + top_k <= 96
-    if (tid < firsts) {
-      const u64 k = keys[(tid / depth) * top_k + tid % depth];
+    if (tid < n_firsts) {
+      const u64 k = firsts[tid];
       int rank = 0;
-      for (int j = 0; j < firsts; ++j) rank += keys[(j / depth) * top_k + j % depth] > k;
+      for (int j = 0; j < n_firsts; j += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const ulonglong2 two = *(const ulonglong2*)(firsts + j + e);
+          rank += (two.x > k) + (two.y > k);
+        }
+      }
       if (rank == top_k - 1 && k) tau = k;
     }
     __syncthreads();
