@@ -21,7 +21,7 @@
  *     scoring targets outside their range are CLAMPED by the kernels (nothing ever indexes outside a table or a
  *     sequence) and reported asynchronously - the NEXT call on the model (or ed_model_check_errors) returns ED_EINVAL
  *     with a message naming what was out of range; the results of the offending call are not valid.  No compute entry
- *     point synchronises the stream.
+ *     point synchronises the stream, but the first ED_PREC_FP8 call on a model, which lays out its weights.
  */
 #ifndef EVODIFF_HIP_H
 #define EVODIFF_HIP_H
@@ -60,7 +60,8 @@ typedef struct ed_config {
   int32_t timesteps;    /* 0 = no timestep encoding (OA-DM); 500 for D3PM (model.py:93-94,133) */
   int32_t activation;   /* 1 = GELU (the only activation on this path), 0 = ReLU.  ED_PREC_FP32 evaluates the exact-erf
                            GELU (erff); ED_PREC_BF16 evaluates x * sigmoid(x (a + b x^2 + c x^4)), a fit of the exact-erf
-                           GELU with at most 2.6e-5 absolute error, ahead of the rounding to bf16 (2^-9 relative) */
+                           GELU with at most 2.6e-5 absolute error, ahead of the rounding to bf16 (2^-9 relative) or,
+                           ED_PREC_FP8, to 8 bits (2^-4) */
   int32_t causal;       /* 0 = MaskedConv1d ('same' padding); 1 = MaskedCausalConv1d, (k-1)*dilation zeros in front
                            only (ByteNetBlock(causal=True), model.py:114: the LR_AR_* models) */
 } ed_config;
