@@ -353,11 +353,26 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 
+// A leaf's accumulation node belongs to the stream of the graph that made it and lives as long as that graph.  A backward pass
+// that is captured on another stream would make that stream wait inside the capture, which the engine's thread does not survive.
+void refuse_foreign_leaf(const at::Tensor& logits) {
+  if (!logits.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(logits);
+  if (!node) return;
+  const c10::Stream now = c10::hip::getCurrentHIPStream(logits.device().index()).unwrap();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing((hipStream_t)current_stream(logits), &status) == hipSuccess, "evodiff_amd: hipStreamIsCapturing failed");
+  const auto made = node->stream();
+  TORCH_CHECK(status == hipStreamCaptureStatusNone || !made.has_value() || *made == now,
+              "evodiff_amd: an eager graph of these logits is alive: let go of its results before a pass with gradients is captured");
+}
+
 Scores token_logprobs_autograd(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     const at::AutoDispatchBelowAutograd below;
     return token_logprobs(logits, targets, select, top_k, n_classes);
   }
+  refuse_foreign_leaf(logits);
   const auto out = TokenLogprobs::apply(logits, targets, select, top_k, n_classes);
   return {out[0], out[1], out[2], out[3]};
 }

@@ -665,6 +665,34 @@ def test_together_captured_and_on_other_streams(dev):
 
 
 @gpu
+def test_capture_with_an_eager_graph_of_the_leaf(dev):
+    """Refused while that graph is alive (only the forward is tried); captured, replayed and right once it is gone."""
+    logits, targets = rand(dev, (40, 700), 3).requires_grad_(), torch.randint(0, 700, (40,), device=dev)
+    ones = torch.ones(40, device=dev)
+
+    def step():
+        out = ops.token_logprobs(logits, targets, 3)
+        return torch.autograd.grad((out.logprob, out.entropy), logits, (ones, ones))[0]
+
+    want = step()
+    alive = ops.token_logprobs(logits, targets, 3)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.token_logprobs(logits, targets, 3)
+    assert torch.equal(torch.autograd.grad((alive.logprob, alive.entropy), logits, (ones, ones))[0], want)
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for _ in range(3):
+        captured.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+        assert torch.equal(step(), want)
+
+
+@gpu
 def test_model_score_tokens(dev):
     """The model's own path: score_tokens agrees with the model's logits in 64 bits and with score_nll, for both precisions."""
     from evodiff_amd.model import ByteNetLMTime
