@@ -621,6 +621,55 @@ def test_long_offsets(dev):
 
 
 @gpu
+def test_linear_long_offsets(dev):
+    """Operands and outputs past 2^32 bytes and elements.  Small whole numbers: exact in 8 bits, every sum exact in fp32."""
+    k, m = 131072, 40008
+    base = torch.randint(-2, 3, (8, k), device=dev).bfloat16()
+    x = torch.empty((m // 8, 8, k), dtype=torch.bfloat16, device=dev)
+    x.copy_(base.expand_as(x))
+    x = x.view(m, k)
+    last = torch.randint(-2, 3, (24, k), device=dev).bfloat16()
+    x[-24:] = last
+    w = torch.randint(-2, 3, (48, k), device=dev).bfloat16()
+    weight = ops.quantize_fp8_weight(w)
+    want, want_last = base.double().cpu() @ w.double().cpu().T, last.double().cpu() @ w.double().cpu().T
+    for rows in (x, ops.quantize_fp8(x)):
+        out = ops.linear_fp8(rows, weight, out_dtype=torch.float32).cpu().double()
+        assert torch.equal(out[-24:], want_last)
+        assert torch.equal(out[:-24].view(-1, 8, 48), want.expand(m // 8 - 3, 8, 48))
+    del x, rows
+    a, b = torch.randint(-3, 4, (66001, 8), device=dev).bfloat16(), torch.randint(-3, 4, (66003, 8), device=dev).bfloat16()
+    out = ops.linear_fp8(a, ops.quantize_fp8_weight(b))  # 4.4e9 values, under 2^8: exact in bf16
+    for rows in (slice(0, 300), slice(65020, 65200), slice(65900, 66001)):
+        assert torch.equal(out[rows].cpu().double(), a[rows].cpu().double() @ b.cpu().double().T)
+
+
+@gpu
+@pytest.mark.parametrize("rows,v", [(70001, 31001), (70000007, 31)])
+def test_log_probabilities_and_gradient_past_32_bits(dev, rows, v):
+    """More than 2^31 logits: the first, middle and last rows as they are alone (fp32 sums in another order: 1e-5 is 80 roundings;
+    gradients rounded to bf16 on both sides: 2^-7)."""
+    some = rand(dev, (1024, v), 1, torch.bfloat16)
+    x = torch.empty((rows, v), dtype=torch.bfloat16, device=dev)
+    for at in range(0, rows, 1024):
+        if v > 100 or at == 0 or at + 1024 >= rows or at % (1 << 20) == 0:
+            x[at:at + 1024] = some[:min(1024, rows - at)]
+    pick = torch.tensor([0, 5, 1 << 16, (1 << 16) + 1, (rows - 1) // 1024 * 1024, rows - 1], device=dev)
+    if v <= 100:
+        pick = torch.tensor([0, 5, 64 << 20, (64 << 20) + 1, (rows - 1) // 1024 * 1024, rows - 1], device=dev)
+    targets = torch.arange(rows, device=dev) % v
+    x.requires_grad_()
+    out = ops.token_logprobs(x, targets, 2)
+    few = x.detach()[pick].requires_grad_()
+    want = ops.token_logprobs(few, targets[pick], 2)
+    for a, b in zip(out, want):
+        assert torch.equal(a[pick], b) if a.dtype == torch.long else torch.allclose(a[pick], b, rtol=1e-5, atol=1e-5)
+    grad, = torch.autograd.grad(out.logprob, x, torch.ones_like(out.logprob))
+    want_grad, = torch.autograd.grad(want.logprob, few, torch.ones_like(want.logprob))
+    assert torch.allclose(grad[pick].float(), want_grad.float(), rtol=2 ** -7, atol=1e-6)
+
+
+@gpu
 def test_together_captured_and_on_other_streams(dev):
     """A scoring step as a program runs it - hidden rows, an 8-bit head, log probabilities, the gradient to the logits - eager,
     in two captured graphs that replay in turn, and on another stream."""
