@@ -453,8 +453,8 @@ __global__ __launch_bounds__(128 * WM, WM / 2) void tile_kernel(Fp8Gemm g, int t
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Few rows (up to 16): the weights are streamed once and bound the time.  A workgroup owns 16 channels, its waves share the
-// blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
+// Few rows (up to 16: the weights are streamed once and bound the time), or little work: latency bounds it.  A workgroup owns
+// 16 rows and 16 channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
 // block's in flight, and brings plain rows to 8 bits in registers - the four lanes that hold a row's block find its
 // largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
 // Measured: 8 x 8192 x 8192 17.2 us, 67 MB of weights at 3.9 TB/s (a copy: 4.7; the start and the join of a single round of
@@ -511,10 +511,10 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
   __shared__ f32x4 sums[16][64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
-  const long n0 = (long)blockIdx.x * 16, pitch = (long)g.kb * FP8_BLOCK;
+  const long n0 = (long)blockIdx.x * 16, m = (long)blockIdx.y * 16 + fr, pitch = (long)g.kb * FP8_BLOCK;
   const long nf = n0 + fr < g.N ? n0 + fr : g.N - 1;  // (channels and rows past the end repeat one that is there, unstored)
-  const bool on = fr < g.M;
-  const long mf = on ? fr : 0;
+  const bool on = m < g.M;
+  const long mf = on ? m : g.M - 1;
   const uint8_t* const w_row = g.wq + nf * pitch + fq * 16;
   const uint8_t* const ws_row = g.ws + (nf >> 7) * g.kb;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -560,7 +560,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
     const long n = n0 + fq * 4 + e;
     if (n >= g.N) break;
     const float y = acc[e] + (g.bias ? g.bias[n] : 0.f);
-    const long o = fr * g.N + n;
+    const long o = m * g.N + n;
     if constexpr (EXACT) ((float*)g.out)[o] = y;
     else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)y;
     else ((_Float16*)g.out)[o] = (_Float16)y;
@@ -714,14 +714,25 @@ static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t strea
   return launch_tile<2, 2, 2, 4, OUT_DT, EXACT>(g, p.parts, stream);
 }
 
-constexpr int FEW_ROWS = 16;
-// Plain rows are brought to 8 bits inside that kernel up to this many blocks of K (every workgroup does it again: 8 x 2560 x
-// 2560 7.6 us against 10.3 us with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3).
-constexpr int FEW_BLOCKS = 24;
+// The few-rows kernel takes up to 16 rows always, and more where 16 x 16 outputs by 128 channels make no more than FEW_WORK pieces
+// and a wave no more than four steps: one launch, no wait between the steps of K.  Sides measured (us, rows already in 8 bits, bf16
+// and fp32 outputs; the tiles need the scales turned first): 32 x 1280 x 1280 6.6 and 6.4, tiles 10.4 and 12.8; 256 x 1280 x 1280
+// (12800 pieces) 8.9 and 10.2, tiles 10.6 and 13.4; 512 x 1280 x 1280 16.2 and 17.2, tiles 10.3 and 13.6.
+constexpr int FEW_ROWS = 16, FEW_WORK = 13000, FEW_K = 64;
+static int64_t few_work(int64_t M, int64_t N, int64_t kb) { return ((M + 15) / 16) * ((N + 15) / 16) * kb; }
+static bool few_rows(int64_t M, int64_t N, int64_t kb) { return M <= FEW_ROWS || (kb <= FEW_K && few_work(M, N, kb) <= FEW_WORK); }
+// Plain rows are brought to 8 bits inside that kernel (every workgroup does it again) up to this many blocks of K (8 x 2560 x 2560
+// 7.6 us against 10.3 with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3) and, beyond 16 rows, pieces (bf16 and fp32: 64 x
+// 1280 x 1280, 3200 pieces, 6.9 and 8.7 against 10.4 and 10.5; 4096 x 31 x 1280, 5120 pieces, 7.1 and 10.0 against 11.2 and 11.6;
+// 128 x 1280 x 1280, 6400 pieces, 9.6 and 12.4 against 10.3 and 10.4).
+constexpr int FEW_BLOCKS = 24, FEW_INSIDE = 5200;
+static bool quantised_inside(int64_t M, int64_t N, int64_t kb) {
+  return kb <= FEW_BLOCKS && (M <= FEW_ROWS || few_work(M, N, kb) <= FEW_INSIDE);
+}
 
 template <int DT>
 static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
-  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
+  const dim3 grid((unsigned)((g.N + 15) / 16), (unsigned)((g.M + 15) / 16)), block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
   if (g.out_dt == DT_FP32) hipLaunchKernelGGL((few_rows_kernel<DT, true>), grid, block, 0, stream, g, r);
   else hipLaunchKernelGGL((few_rows_kernel<DT, false>), grid, block, 0, stream, g, r);
   return hipGetLastError();
@@ -762,18 +773,18 @@ static int64_t scales_end(int64_t M, int64_t kb, bool quantised) {
 }
 int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact) {
   const int64_t kb = fp8_blocks(K);
-  if (M <= FEW_ROWS) return quantised || kb <= FEW_BLOCKS ? 0 : M * kb * (FP8_BLOCK + 1);
+  if (few_rows(M, N, kb)) return quantised || quantised_inside(M, N, kb) ? 0 : M * kb * (FP8_BLOCK + 1);
   const Plan p = plan_of(M, N, (int)kb, exact);
   return scales_end(M, kb, quantised) + (p.parts > 1 ? p.parts * M * N * 4 : 0);
 }
 
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   const int kb = (int)fp8_blocks(p.K);
-  if (p.M <= FEW_ROWS) {
+  if (few_rows(p.M, p.N, kb)) {
     const Fp8Gemm g{nullptr, nullptr, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
     FewRows r{p.x, (long)p.row_stride, (long)p.K, p.x_scale, p.x_dt != DT_E4M3 && wide_rows(p.x, p.x_dt, p.row_stride)};
     if (p.x_dt != DT_E4M3) {
-      if (kb <= FEW_BLOCKS) {
+      if (quantised_inside(p.M, p.N, kb)) {
         if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, stream);
         if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, stream);
         return launch_few_rows<DT_FP16>(g, r, stream);
