@@ -454,7 +454,7 @@ __global__ __launch_bounds__(128 * WM, WM / 2) void tile_kernel(Fp8Gemm g, int t
 
 // ---------------------------------------------------------------------------------------------------
 // Few rows (up to 16: the weights are streamed once and bound the time), or little work: latency bounds it.  A workgroup owns
-// 16 rows and 16 channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
+// 16 rows and 16 NF channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
 // block's in flight, and brings plain rows to 8 bits in registers - the four lanes that hold a row's block find its
 // largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
 // Measured: 8 x 8192 x 8192 17.2 us, 67 MB of weights at 3.9 TB/s (a copy: 4.7; the start and the join of a single round of
@@ -506,25 +506,34 @@ struct FewRows {
   bool wide;
 };
 
-template <int DT, bool EXACT>
+template <int DT, bool EXACT, int NF>
 __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
-  __shared__ f32x4 sums[16][64];
+  __shared__ f32x4 sums[16][NF][64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
-  const long n0 = (long)blockIdx.x * 16, m = (long)blockIdx.y * 16 + fr, pitch = (long)g.kb * FP8_BLOCK;
-  const long nf = n0 + fr < g.N ? n0 + fr : g.N - 1;  // (channels and rows past the end repeat one that is there, unstored)
+  const long n0 = (long)blockIdx.x * 16 * NF, m = (long)blockIdx.y * 16 + fr, pitch = (long)g.kb * FP8_BLOCK;
+  // (channels and rows past the end repeat one that is there, unstored)
   const bool on = m < g.M;
   const long mf = on ? m : g.M - 1;
-  const uint8_t* const w_row = g.wq + nf * pitch + fq * 16;
-  const uint8_t* const ws_row = g.ws + (nf >> 7) * g.kb;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  i32x4 w_next[2];
-  int sw_next;
+  const uint8_t *w_row[NF], *ws_row[NF];
+  f32x4 acc[NF];
+  i32x4 w_next[NF][2];
+  int sw_next[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const long n = n0 + 16 * f + fr, nf = n < g.N ? n : g.N - 1;
+    w_row[f] = g.wq + nf * pitch + fq * 16;
+    ws_row[f] = g.ws + (nf >> 7) * g.kb;
+    acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   auto fetch = [&](int b) {
     if (b >= g.kb) return;
-    w_next[0] = *(const i32x4*)(w_row + (long)b * FP8_BLOCK);
-    w_next[1] = *(const i32x4*)(w_row + (long)b * FP8_BLOCK + 64);
-    sw_next = ws_row[b];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      w_next[f][0] = *(const i32x4*)(w_row[f] + (long)b * FP8_BLOCK);
+      w_next[f][1] = *(const i32x4*)(w_row[f] + (long)b * FP8_BLOCK + 64);
+      sw_next[f] = ws_row[f][b];
+    }
   };
   fetch(wid);
   for (int b = wid; b < g.kb; b += waves) {
@@ -539,31 +548,43 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
       part.load(r.x, mf * r.row_stride, (long)b * FP8_BLOCK + fq * 16, r.K, on, r.wide);
       sx = part.quantise(X);
     }
-    const i32x8 W = __builtin_shufflevector(w_next[0], w_next[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    const int sw = sw_next;
-    fetch(b + waves);
-    if constexpr (EXACT) {
-      f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    i32x8 W[NF];
+    int sw[NF];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(W, h), widen(X, h), part, 0, 0, 0);
-      add_scaled(acc, part, sx, sw);
-    } else {
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W, X, acc, 0, 0, 0, sw, 0, sx);
+    for (int f = 0; f < NF; ++f) {
+      W[f] = __builtin_shufflevector(w_next[f][0], w_next[f][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      sw[f] = sw_next[f];
+    }
+    fetch(b + waves);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      if constexpr (EXACT) {
+        f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(W[f], h), widen(X, h), part, 0, 0, 0);
+        add_scaled(acc[f], part, sx, sw[f]);
+      } else {
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W[f], X, acc[f], 0, 0, 0, sw[f], 0, sx);
+      }
     }
   }
-  sums[wid][lane] = acc;
-  __syncthreads();
-  if (tid >= 64 || !on) return;
-  for (int w = 1; w < waves; ++w) acc += sums[w][lane];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const long n = n0 + fq * 4 + e;
-    if (n >= g.N) break;
-    const float y = acc[e] + (g.bias ? g.bias[n] : 0.f);
-    const long o = m * g.N + n;
-    if constexpr (EXACT) ((float*)g.out)[o] = y;
-    else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)y;
-    else ((_Float16*)g.out)[o] = (_Float16)y;
+  for (int f = 0; f < NF; ++f) sums[wid][f][lane] = acc[f];
+  __syncthreads();
+  for (int j = wid; j < NF; j += waves) {  // wave j joins fragment j
+    if (!on) break;
+    f32x4 y = sums[0][j][lane];
+    for (int w = 1; w < waves; ++w) y += sums[w][j][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long n = n0 + 16 * j + fq * 4 + e;
+      if (n >= g.N) break;
+      const float v = y[e] + (g.bias ? g.bias[n] : 0.f);
+      const long o = m * g.N + n;
+      if constexpr (EXACT) ((float*)g.out)[o] = v;
+      else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)v;
+      else ((_Float16*)g.out)[o] = (_Float16)v;
+    }
   }
 }
 
@@ -716,26 +737,36 @@ static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t strea
 
 // The few-rows kernel takes up to 16 rows always, and more where 16 x 16 outputs by 128 channels make no more than FEW_WORK pieces
 // and a wave no more than four steps: one launch, no wait between the steps of K.  Sides measured (us, rows already in 8 bits, bf16
-// and fp32 outputs; the tiles need the scales turned first): 32 x 1280 x 1280 6.6 and 6.4, tiles 10.4 and 12.8; 256 x 1280 x 1280
-// (12800 pieces) 8.9 and 10.2, tiles 10.6 and 13.4; 512 x 1280 x 1280 16.2 and 17.2, tiles 10.3 and 13.6.
-constexpr int FEW_ROWS = 16, FEW_WORK = 13000, FEW_K = 64;
+// and fp32 outputs; the tiles need the scales turned first): 64 x 1280 x 1280 6.8 and 6.4, tiles 10.6 and 13.3; 300 x 1111 x 1000
+// (10640 pieces) 8.4 and 9.1, tiles 10.6 and 13.4; plain rows there 11.2 and 11.7, tiles 10.6 and 13.8; 1024 x 640 x 640 (12800) 12.4
+// and 13.1, tiles 10.3 and 10.4.
+constexpr int FEW_ROWS = 16, FEW_WORK = 11000, FEW_K = 64;
 static int64_t few_work(int64_t M, int64_t N, int64_t kb) { return ((M + 15) / 16) * ((N + 15) / 16) * kb; }
 static bool few_rows(int64_t M, int64_t N, int64_t kb) { return M <= FEW_ROWS || (kb <= FEW_K && few_work(M, N, kb) <= FEW_WORK); }
 // Plain rows are brought to 8 bits inside that kernel (every workgroup does it again) up to this many blocks of K (8 x 2560 x 2560
-// 7.6 us against 10.3 with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3) and, beyond 16 rows, pieces (bf16 and fp32: 64 x
-// 1280 x 1280, 3200 pieces, 6.9 and 8.7 against 10.4 and 10.5; 4096 x 31 x 1280, 5120 pieces, 7.1 and 10.0 against 11.2 and 11.6;
-// 128 x 1280 x 1280, 6400 pieces, 9.6 and 12.4 against 10.3 and 10.4).
-constexpr int FEW_BLOCKS = 24, FEW_INSIDE = 5200;
+// 7.6 us against 10.3 with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3) and, beyond 16 rows, pieces (bf16 and fp32: 4096 x
+// 31 x 1280, 5120 pieces, 6.6 and 6.7 against 10.0 and 10.4; 128 x 640 x 2560, 6400 pieces, 7.8 and 10.3 against 10.2 and 10.4;
+// 300 x 1111 x 1000, 10640 pieces, 10.0 and 11.2 against 10.4 and 11.0).
+constexpr int FEW_BLOCKS = 24, FEW_INSIDE = 8000;
 static bool quantised_inside(int64_t M, int64_t N, int64_t kb) {
   return kb <= FEW_BLOCKS && (M <= FEW_ROWS || few_work(M, N, kb) <= FEW_INSIDE);
 }
 
+template <int DT, int NF>
+static hipError_t launch_few(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
+  const dim3 grid((unsigned)((g.N + 16 * NF - 1) / (16 * NF)), (unsigned)((g.M + 15) / 16));
+  const dim3 block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
+  if (g.out_dt == DT_FP32) hipLaunchKernelGGL((few_rows_kernel<DT, true, NF>), grid, block, 0, stream, g, r);
+  else hipLaunchKernelGGL((few_rows_kernel<DT, false, NF>), grid, block, 0, stream, g, r);
+  return hipGetLastError();
+}
+// 16 channels a workgroup, so that as many as there can be read the weights (8 x 8192 x 8192 17.7 us against 18.5 with 32); 32 where
+// more than 16 rows are brought to 8 bits inside, which each workgroup does (128 x 1280 x 1280 8.6 us against 9.5).
 template <int DT>
 static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
-  const dim3 grid((unsigned)((g.N + 15) / 16), (unsigned)((g.M + 15) / 16)), block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
-  if (g.out_dt == DT_FP32) hipLaunchKernelGGL((few_rows_kernel<DT, true>), grid, block, 0, stream, g, r);
-  else hipLaunchKernelGGL((few_rows_kernel<DT, false>), grid, block, 0, stream, g, r);
-  return hipGetLastError();
+  if constexpr (DT != DT_E4M3)
+    if (g.M > FEW_ROWS) return launch_few<DT, 2>(g, r, stream);
+  return launch_few<DT, 1>(g, r, stream);
 }
 
 template <int OUT_DT>
