@@ -726,10 +726,11 @@ __device__ __forceinline__ float named(const int64_t* targets, int top_k, const 
   return d;
 }
 
-// A workgroup per `per` tiles of 256 vectors of a row: 16-byte loads, the next tile's in flight, and 16-byte stores where source
-// and destination rows lie alike within 16 bytes; class by class elsewhere.  The stores pass by the caches (the reader behind is a
-// product over the whole gradient): 4096 x 32000 bf16 117 -> 90 us (5.8 TB/s in and out), 1024 x 32000 fp32 56 -> 43.  The named classes of the piece are
-// listed in shared memory while the first loads fly, with a bit for each vector that holds one.
+// A workgroup per `per` tiles of 256 vectors of a row, 16 bytes of the destination each: loads, the next tile's in flight, at whatever
+// alignment the source has there (the last 32000 of 32001 columns, 4096 rows, bf16: 99 us, class by class 295), and aligned stores.
+// The stores pass by the caches (the reader behind is a product over the whole gradient): 4096 x 32000 bf16 117 -> 90 us (5.8 TB/s
+// in and out), 1024 x 32000 fp32 56 -> 43.  The named classes of the piece are listed in shared memory while the first loads fly,
+// with a bit for each vector that holds one.
 constexpr int GRAD_TILES = 8;  // at most, of a workgroup
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const int64_t* __restrict__ targets,
@@ -738,6 +739,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
   typedef typename Elem<DT>::T T;
   constexpr int EPV = 16 / sizeof(T), U = 2;
   typedef __attribute__((ext_vector_type(EPV))) T VT;
+  typedef VT Loose __attribute__((aligned(sizeof(T))));
   __shared__ int64_t cls[TOP_MAX + 1];  // named classes and their gradients, in order
   __shared__ float cls_g[TOP_MAX + 1];
   __shared__ int name_at[TOP_MAX + 1];  // those of this piece, each once, and their sums
@@ -752,16 +754,15 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
     const T* row = row_of<T>(x, r);
     T* dst = (T*)g.dlogits + r * g.columns;
     const int head = (int)((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / (int)sizeof(T);
-    const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
     // the vectors of this piece, all of them classes; columns beside vectors are the first and the last piece's
-    const int vectors = alike && x.n > head ? (x.n - head) / EPV : 0;
+    const int vectors = x.n > head ? (x.n - head) / EPV : 0;
     const int v0 = piece * per * 256 < vectors ? piece * per * 256 : vectors;
     const int v1 = v0 + per * 256 < vectors && piece + 1 < pieces ? v0 + per * 256 : vectors;
     uint4 next[U];
     auto load = [&](int at) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (at + u * 256 + tid < v1) next[u] = *(const uint4*)(row + head + (long)(at + u * 256 + tid) * EPV);
+        if (at + u * 256 + tid < v1) next[u] = __builtin_bit_cast(uint4, *(const Loose*)(row + head + (long)(at + u * 256 + tid) * EPV));
     };
     load(v0);
     GradRow a = grad_row(x, targets, select, g, r);
