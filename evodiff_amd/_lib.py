@@ -10,6 +10,7 @@ LIB_PATH = os.environ.get("EVODIFF_AMD_LIB") or os.path.join(_HERE, "csrc", "lib
 
 PREC_FP32, PREC_BF16, PREC_FP8 = 0, 1, 2
 DT_FP32, DT_BF16, DT_FP16, DT_E4M3 = 0, 1, 2, 3
+FAST_SUMS = 0x100
 TOP_K_MAX = 32
 K_EMBED, K_LNACT, K_GEMM1X1, K_CONV, K_FINAL, K_CONV_OTHER, K_COUNT = 0, 1, 2, 3, 4, 5, 6
 KIND_NAMES = ("embed", "ln_act", "gemm1x1", "conv", "final", "conv_other")

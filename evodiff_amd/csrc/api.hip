@@ -1722,13 +1722,14 @@ int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, i
 
 int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype, int out_dtype) {
   if (M < 1 || N < 1 || K < 1 || M >= MAX_DIM || N >= MAX_DIM || K > MAX_K) return 0;
-  return fp8_linear_workspace(M, N, K, x_dtype == ED_DT_E4M3, out_dtype == ED_DT_FP32);
+  return fp8_linear_workspace(M, N, K, x_dtype == ED_DT_E4M3, !(out_dtype & ED_FAST_SUMS));
 }
 
 int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
                   const uint8_t* weight_scale_dev, const float* bias_dev, void* out_dev, int out_dtype, int64_t M, int64_t N,
                   int64_t K, void* workspace_dev, int64_t workspace_bytes, void* stream) {
-  const bool quantised = x_dtype == ED_DT_E4M3;
+  const bool quantised = x_dtype == ED_DT_E4M3, fast = (out_dtype & ED_FAST_SUMS) != 0;
+  out_dtype &= ~ED_FAST_SUMS;
   if (quantised) {
     if (M < 0 || M >= MAX_DIM || K < 1 || K > MAX_K || fp8_blocks(K) * M >= MAX_BLOCKS)
       return fail(ED_EINVAL, "x: %lld x %lld values are out of range", (long long)M, (long long)K);
@@ -1738,6 +1739,7 @@ int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint
     return rc;
   }
   if (!plain_dtype(out_dtype)) return fail(ED_EINVAL, "out: dtype must be fp32, bf16 or fp16 (got %d)", out_dtype);
+  if (fast && out_dtype == ED_DT_FP32) return fail(ED_EINVAL, "ED_FAST_SUMS is for bf16 and fp16 outputs: an fp32 output has fp32 sums");
   if (N < 1 || N >= MAX_DIM || fp8_blocks(K) * N >= MAX_BLOCKS) return fail(ED_EINVAL, "weight: %lld x %lld values are out of range", (long long)N, (long long)K);
   if (((M + 15) / 16) * ((N + 15) / 16) >= MAX_BLOCKS) return fail(ED_EINVAL, "out: %lld x %lld values are out of range", (long long)M, (long long)N);
   if (M == 0) return ED_OK;
@@ -1745,11 +1747,11 @@ int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint
     return fail(ED_EINVAL, "null x/scale/weight/out pointer");
   if (misaligned(weight_dev, 16)) return fail(ED_EINVAL, "the weight must be aligned to 16 bytes");
   if (misaligned(out_dev, (size_t)dt_bytes(out_dtype)) || misaligned(bias_dev, 4)) return fail(ED_EINVAL, "out/bias: not aligned to their element");
-  const int64_t need = fp8_linear_workspace(M, N, K, quantised, out_dtype == ED_DT_FP32);
+  const int64_t need = fp8_linear_workspace(M, N, K, quantised, !fast);
   if (need > 0 && (!workspace_dev || workspace_bytes < need || misaligned(workspace_dev, 16)))
     return fail(ED_EINVAL, "workspace: %lld bytes at a 16-byte boundary are needed (ed_fp8_linear_workspace)", (long long)need);
   const Fp8Linear p{x_dev, x_dtype, row_stride, x_scale_dev, weight_dev, weight_scale_dev, bias_dev, out_dev, out_dtype,
-                    M, N, K, workspace_dev};
+                    M, N, K, workspace_dev, fast};
   LAUNCH_TRY(launch_fp8_linear(p, (hipStream_t)stream));
   return ED_OK;
 }

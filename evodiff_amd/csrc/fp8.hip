@@ -118,9 +118,10 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const void* __rest
 
 
 // Eight products at a time, the 8-bit matrix instructions (scaled or not, any shape) align to the largest and drop what lies
-// under 2^-13 of it: results are 4e-5 to 6e-5 (2-norm) from the exact sum at any K, well under half a step of bf16 (2e-3) or fp16
-// (2e-4), which those outputs are rounded by anyway.  fp32 outputs take the exact form: e4m3 values are exact in bf16, so are
-// their products in fp32, and the bf16 instruction keeps fp32 sums; it has half the rate.
+// under 2^-13 of it: results are 4e-5 to 6e-5 (2-norm) from the exact sum at any K, and where a large product cancels against
+// another group's, what stood beside it is gone.  So a product takes the exact form, whatever its output's type: e4m3 values are exact in
+// bf16, so are their products in fp32, and the bf16 instruction, at half the rate, keeps fp32 sums.  The 8-bit instruction is for
+// callers that ask for it: ED_FAST_SUMS, and the model at ED_PREC_FP8, whose operands' rounding (3 % a product) is far above it.
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 
 // values 8 s2 .. 8 s2 + 7 of a fragment as bf16 (exact: the upper halves of their fp32 forms; a NaN stays one).  Four full-rate
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(Fp8Gemm g, FewRows r) {
       if (n >= g.N) break;
       const float v = y[e] + (g.bias ? g.bias[n] : 0.f);
       const long o = m * g.N + n;
-      if constexpr (EXACT) ((float*)g.out)[o] = v;
+      if (g.out_dt == DT_FP32) ((float*)g.out)[o] = v;
       else if (g.out_dt == DT_BF16) ((__bf16*)g.out)[o] = (__bf16)v;
       else ((_Float16*)g.out)[o] = (_Float16)v;
     }
@@ -752,25 +753,24 @@ static bool quantised_inside(int64_t M, int64_t N, int64_t kb) {
 }
 
 template <int DT, int NF>
-static hipError_t launch_few(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
+static hipError_t launch_few(const Fp8Gemm& g, const FewRows& r, bool exact, hipStream_t stream) {
   const dim3 grid((unsigned)((g.N + 16 * NF - 1) / (16 * NF)), (unsigned)((g.M + 15) / 16));
   const dim3 block(64 * (g.kb < 16 ? g.kb : 16));  // (no wave without a block of K)
-  if (g.out_dt == DT_FP32) hipLaunchKernelGGL((few_rows_kernel<DT, true, NF>), grid, block, 0, stream, g, r);
+  if (exact) hipLaunchKernelGGL((few_rows_kernel<DT, true, NF>), grid, block, 0, stream, g, r);
   else hipLaunchKernelGGL((few_rows_kernel<DT, false, NF>), grid, block, 0, stream, g, r);
   return hipGetLastError();
 }
 // 16 channels a workgroup, so that as many as there can be read the weights (8 x 8192 x 8192 17.7 us against 18.5 with 32); 32 where
 // more than 16 rows are brought to 8 bits inside, which each workgroup does (128 x 1280 x 1280 8.6 us against 9.5).
 template <int DT>
-static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, hipStream_t stream) {
+static hipError_t launch_few_rows(const Fp8Gemm& g, const FewRows& r, bool exact, hipStream_t stream) {
   if constexpr (DT != DT_E4M3)
-    if (g.M > FEW_ROWS) return launch_few<DT, 2>(g, r, stream);
-  return launch_few<DT, 1>(g, r, stream);
+    if (g.M > FEW_ROWS) return launch_few<DT, 2>(g, r, exact, stream);
+  return launch_few<DT, 1>(g, r, exact, stream);
 }
 
-template <int OUT_DT>
+template <int OUT_DT, bool EXACT>
 static hipError_t launch_gemm(const Fp8Gemm& g, void* partial, hipStream_t stream) {
-  constexpr bool EXACT = OUT_DT == DT_FP32;
   const Plan p = plan_of(g.M, g.N, g.kb, EXACT);
   if (p.parts == 1) return launch_plan<OUT_DT, EXACT>(g, p, stream);
   Fp8Gemm part = g;
@@ -810,14 +810,15 @@ int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bo
 
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   const int kb = (int)fp8_blocks(p.K);
+  const bool exact = !p.fast;
   if (few_rows(p.M, p.N, kb)) {
     const Fp8Gemm g{nullptr, nullptr, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
     FewRows r{p.x, (long)p.row_stride, (long)p.K, p.x_scale};
     if (p.x_dt != DT_E4M3) {
       if (quantised_inside(p.M, p.N, kb)) {
-        if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, stream);
-        if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, stream);
-        return launch_few_rows<DT_FP16>(g, r, stream);
+        if (p.x_dt == DT_FP32) return launch_few_rows<DT_FP32>(g, r, exact, stream);
+        if (p.x_dt == DT_BF16) return launch_few_rows<DT_BF16>(g, r, exact, stream);
+        return launch_few_rows<DT_FP16>(g, r, exact, stream);
       }
       uint8_t* const q = (uint8_t*)p.workspace;
       uint8_t* const scale = q + p.M * kb * FP8_BLOCK;
@@ -826,7 +827,7 @@ hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
       r.x = q;
       r.x_scale = scale;
     }
-    return launch_few_rows<DT_E4M3>(g, r, stream);
+    return launch_few_rows<DT_E4M3>(g, r, exact, stream);
   }
   const uint8_t* xq = (const uint8_t*)p.x;
   uint8_t* xs = (uint8_t*)p.workspace;
@@ -844,9 +845,9 @@ hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream) {
   if (e != hipSuccess) return e;
   const Fp8Gemm g{xq, xs, p.w, p.w_scale, p.bias, p.out, p.out_dt, p.M, p.N, kb};
   void* const partial = (char*)p.workspace + scales_end(p.M, kb, p.x_dt == DT_E4M3);
-  if (p.out_dt == DT_FP32) return launch_gemm<DT_FP32>(g, partial, stream);
-  if (p.out_dt == DT_BF16) return launch_gemm<DT_BF16>(g, partial, stream);
-  return launch_gemm<DT_FP16>(g, partial, stream);
+  if (p.out_dt == DT_FP32) return exact ? launch_gemm<DT_FP32, true>(g, partial, stream) : hipErrorInvalidValue;
+  if (p.out_dt == DT_BF16) return exact ? launch_gemm<DT_BF16, true>(g, partial, stream) : launch_gemm<DT_BF16, false>(g, partial, stream);
+  return exact ? launch_gemm<DT_FP16, true>(g, partial, stream) : launch_gemm<DT_FP16, false>(g, partial, stream);
 }
 
 }  // namespace ed

@@ -58,8 +58,9 @@ struct Fp8Linear {
   int out_dt;
   int64_t M, N, K;
   void* workspace;  // fp8_linear_workspace bytes, 16-byte aligned
+  bool fast;        // sums as the 8-bit instruction takes them (16-bit outputs only), else fp32
 };
-int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact);  // exact: fp32 output
+int64_t fp8_linear_workspace(int64_t M, int64_t N, int64_t K, bool quantised, bool exact);  // exact: not fast
 hipError_t launch_fp8_linear(const Fp8Linear& p, hipStream_t stream);
 
 // Rows of logits: row r = (o, i) = (r / inner, r % inner) starts at o * outer_stride + i * inner_stride (elements).

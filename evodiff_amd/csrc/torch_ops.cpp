@@ -164,7 +164,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8_weight(const at::Tensor& w) { re
 
 at::Tensor linear_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& x_scale, const at::Tensor& weight,
                       const at::Tensor& weight_scale, const c10::optional<at::Tensor>& bias,
-                      c10::optional<at::ScalarType> out_dtype) {
+                      c10::optional<at::ScalarType> out_dtype, bool fast_sums) {
   want(weight, at::kFloat8_e4m3fn, "weight.q");
   want(weight_scale, at::kFloat8_e8m0fnu, "weight.scale");
   same_device(weight, x, "x");
@@ -192,18 +192,20 @@ at::Tensor linear_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& x_sc
   }
   const at::ScalarType ot = out_dtype.has_value() ? *out_dtype : x_scale.has_value() ? at::kBFloat16 : x.scalar_type();
   TORCH_CHECK(ot == at::kFloat || ot == at::kBFloat16 || ot == at::kHalf, "evodiff_amd: out_dtype must be float32, bfloat16 or float16, got ", ot);
+  TORCH_CHECK(!fast_sums || ot != at::kFloat, "evodiff_amd: fast_sums is for bfloat16 and float16 outputs: a float32 output has float32 sums");
   const c10::DeviceGuard guard(x.device());
   const at::Tensor r = as_rows(x, "x");
   const int64_t M = r.size(0), K = r.size(1);
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = N;
   at::Tensor out = at::empty(shape, x.options().dtype(ot));
-  const int64_t need = ed_fp8_linear_workspace(M, N, K, dt, dtype_of(out, "out"));
+  const int out_code = dtype_of(out, "out") | (fast_sums ? ED_FAST_SUMS : 0);
+  const int64_t need = ed_fp8_linear_workspace(M, N, K, dt, out_code);
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, x.options().dtype(at::kByte));
   check(ed_fp8_linear(r.data_ptr(), dt, r.stride(0), ptr_or_null<uint8_t>(x_scale), (const uint8_t*)weight.data_ptr(),
-                      (const uint8_t*)weight_scale.data_ptr(), ptr_or_null<float>(bias), out.data_ptr(), dtype_of(out, "out"), M, N,
-                      K, need > 0 ? ws.data_ptr() : nullptr, need, current_stream(x)));
+                      (const uint8_t*)weight_scale.data_ptr(), ptr_or_null<float>(bias), out.data_ptr(), out_code, M, N, K,
+                      need > 0 ? ws.data_ptr() : nullptr, need, current_stream(x)));
   return out;
 }
 
@@ -386,7 +388,7 @@ TORCH_LIBRARY(evodiff_amd, m) {
   m.def("score_nll(int handle, Tensor tokens, Tensor timesteps, Tensor targets, Tensor? select, int n_classes, int precision) -> Tensor");
   m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)");
   m.def("quantize_fp8_weight(Tensor w) -> (Tensor, Tensor)");
-  m.def("linear_fp8(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType? out_dtype) -> Tensor");
+  m.def("linear_fp8(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType? out_dtype, bool fast_sums=False) -> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor? targets, Tensor? select, int top_k, int n_classes) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 

@@ -44,7 +44,7 @@ enum {
 
 /* ED_PREC_FP8 (ed_forward, ed_forward_collect, ed_score_nll, ed_score_tokens): every product of the block stack takes both
  * operands in the block-scaled 8-bit form described at ed_fp8_quantize_rows (weights are laid out at the first such call, which
- * synchronises once); LayerNorms, the residual stream and all sums stay fp32, the vocabulary projection fp32. */
+ * synchronises once), summed as ED_FAST_SUMS says; LayerNorms, the residual stream and the vocabulary projection stay fp32. */
 enum { ED_PREC_FP32 = 0, ED_PREC_BF16 = 1, ED_PREC_FP8 = 2 };
 
 /* Hyper-parameters of ByteNetLMTime as constructed by evodiff/pretrained.py:39-42 from
@@ -285,11 +285,15 @@ int ed_fp8_quantize_weight(const void* w_dev, int w_dtype, int64_t row_stride, i
                            uint8_t* scale_dev, void* stream);
 
 /* out (M, N) = x (M, K) @ weight (N, K)^T + bias, sums in fp32, rounded once to out_dtype (FP32, BF16 or FP16; contiguous).
+ * out_dtype | ED_FAST_SUMS (BF16 or FP16): sums as the 8-bit matrix instruction takes them, for up to three times the rate of large
+ * products.  Of eight neighbouring products the bits under 2^-13 of the largest are dropped, so a sum is off by up to 7 * 2^-13
+ * of its terms' magnitudes (4e-5 to 6e-5 in 2-norm on ordinary data); where large terms cancel, that is more than the rounding.
  * x_dtype ED_DT_E4M3: x_dev and x_scale_dev are rows in the form above (row_stride = Kb * 128).  Any other x_dtype: x_dev holds
  * plain values, which are brought to that form first (x_scale_dev is ignored) - the result is the same, bit for bit, as
  * of ed_fp8_quantize_rows and a product on its outputs.  bias_dev: fp32 [N] or NULL.
  * workspace_dev: at least ed_fp8_linear_workspace(M, N, K, x_dtype, out_dtype) bytes, 16-byte aligned (NULL where that is 0); its contents
  * do not matter before or after the call. */
+#define ED_FAST_SUMS 0x100
 int64_t ed_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int x_dtype, int out_dtype);
 int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint8_t* x_scale_dev, const uint8_t* weight_dev,
                   const uint8_t* weight_scale_dev, const float* bias_dev, void* out_dev, int out_dtype, int64_t M, int64_t N,

@@ -1,0 +1,99 @@
+"""What the interface of the model-free operators (evodiff_amd.ops) promises beside the plain cases: fp32 sums whatever the output's
+type, no derivative that is lost without a word, the widths of operands, rows that are left out, targets that are none.
+
+Tolerances are derived where they stand; a rounding is off by at most ``torch.finfo(t).eps / 2`` of the value.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from evodiff_amd import _lib, ops
+from test_ops import (DTYPES, HALF, SHAPES, TILES, check_product, dequantized, dev, logprob_tolerance, plain_grad,  # noqa: F401
+                      plain_logprobs, plain_quantize, rand, rel_ok)
+
+gpu = pytest.mark.gpu
+HALVES = [torch.bfloat16, torch.float16]
+
+
+# ---- sums of a product -----------------------------------------------------------------------------------------------
+
+# every form of the product: few rows (quantised inside and before), little work, tiles of 64 and 128, a cut K loop, many rows
+FORMS = [(1, 16, 128), (3, 300, 1280), (8, 2048, 4096), (40, 64, 640), (300, 1000, 1111), (200, 1280, 1280), (130, 3588, 4200),
+         (2572, 1302, 32), (5000, 2560, 128), (16384, 1280, 256)]
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", FORMS)
+@pytest.mark.parametrize("out_dtype", HALVES)
+def test_linear_keeps_small_products_beside_large_ones_that_cancel(dev, m, n, k, out_dtype):
+    """448 * 448 and its negative eight columns on, seven small products beside the first: whole numbers under 2^24, so that fp32 sums
+    are exact in any order, and a result of at most 84, exact in every type."""
+    x, w = torch.zeros((m, k), device=dev), torch.zeros((n, k), device=dev)
+    a, b = 1 + torch.arange(m, device=dev) % 4, 1 + torch.arange(n, device=dev) % 3
+    x[:, 0], x[:, 8], x[:, 1:8] = 448.0, -448.0, a[:, None].float()
+    w[:, 0], w[:, 8], w[:, 1:8] = 448.0, 448.0, b[:, None].float()
+    want = (7 * a[:, None] * b).to(out_dtype)
+    weight = ops.quantize_fp8_weight(w)
+    for rows in (x.to(out_dtype), x, ops.quantize_fp8(x)):
+        assert torch.equal(ops.linear_fp8(rows, weight, out_dtype=out_dtype), want)
+
+
+def check_sums(x, w, bias, got):
+    """As ``check_product``, with fp32 sums for every output type: at most 128 Kb + 1 additions, each off by 2^-24 of the sum of
+    magnitudes, then one rounding."""
+    xd, wd = dequantized(*plain_quantize(x, False), False), dequantized(*plain_quantize(w, True), True)
+    want, size = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if bias is not None:
+        want, size = want + bias.cpu().double(), size + bias.cpu().double().abs()
+    sums = (xd.shape[1] + 2) * 2.0 ** -24 * size
+    off = (got.cpu().double() - want).abs() - (sums + (want.abs() + sums) * HALF[got.dtype] + 2.0 ** -25)
+    assert float(off.max()) <= 0, float(off.max())
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("out_dtype", HALVES)
+def test_linear_of_16_bit_outputs_against_fp32_sums(dev, m, n, k, out_dtype):
+    x, w = rand(dev, (m, k), m + n, out_dtype, 1.0), rand(dev, (n, k), m + k, torch.float32) / k ** 0.5
+    bias = rand(dev, (n,), 3) if (m + n) % 2 else None
+    check_sums(x, w, bias, ops.linear_fp8(x, ops.quantize_fp8_weight(w), bias))
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", SHAPES + TILES)
+@pytest.mark.parametrize("out_dtype", HALVES)
+def test_linear_fast_sums(dev, m, n, k, out_dtype):
+    """The 8-bit instruction's sums, where they are asked for: seven of eight products lose less than 2^-13 of the largest each."""
+    x, w = rand(dev, (m, k), m + n, out_dtype, 1.0), rand(dev, (n, k), m + k, torch.float32) / k ** 0.5
+    bias = rand(dev, (n,), 3) if (m + n) % 2 else None
+    weight = ops.quantize_fp8_weight(w)
+    got = ops.linear_fp8(x, weight, bias, fast_sums=True)
+    rows = torch.arange(m) if m <= 512 else torch.cat([torch.arange(160), torch.arange(160) + m // 2 - 80, torch.arange(m - 160, m)])
+    check_product(dev, x[rows.to(dev)], w, bias, out_dtype, got[rows.to(dev)])
+    # every row: two sums of the same products, off by at most the above; then a rounding each
+    exact = ops.linear_fp8(x, weight, bias, out_dtype=torch.float32)
+    assert float((got.float() - exact).norm() / exact.norm()) < 2.0 ** -12 + HALF[out_dtype]
+    assert torch.equal(got, ops.linear_fp8(ops.quantize_fp8(x), weight, bias, out_dtype=out_dtype, fast_sums=True))
+
+
+@gpu
+def test_linear_fast_sums_are_for_16_bit_outputs(dev):
+    x, w = rand(dev, (4, 256), 1), ops.quantize_fp8_weight(rand(dev, (64, 256), 0))
+    with pytest.raises(RuntimeError, match="float32 output"):
+        ops.linear_fp8(x, w, fast_sums=True)
+    assert ops.linear_fp8(x, w, out_dtype=torch.bfloat16, fast_sums=True).dtype == torch.bfloat16
+
+
+def test_fast_sums_of_the_c_entry_point():
+    lib, p = _lib.load(), ctypes.c_void_p(1 << 20)      # never read: the call is refused on the host
+    assert lib.ed_fp8_linear(p, 1, 256, None, p, p, None, p, _lib.DT_FP32 | _lib.FAST_SUMS, 4, 8, 256, p, 1 << 20, None) == -1
+    assert "ED_FAST_SUMS" in lib.ed_last_error().decode()
+    assert lib.ed_fp8_linear(p, 1, 256, None, p, p, None, p, _lib.DT_E4M3 | _lib.FAST_SUMS, 4, 8, 256, p, 1 << 20, None) == -1
+    assert "dtype" in lib.ed_last_error().decode()
+    for out in (_lib.DT_BF16, _lib.DT_BF16 | _lib.FAST_SUMS):    # each form has its own workspace, and refuses less
+        need = lib.ed_fp8_linear_workspace(4096, 4096, 4096, _lib.DT_BF16, out)
+        assert need >= 4096 * 32 * 129
+        assert lib.ed_fp8_linear(p, 1, 4096, None, p, p, None, p, out, 4096, 4096, 4096, p, need - 1, None) == -1
+        assert "workspace" in lib.ed_last_error().decode()
