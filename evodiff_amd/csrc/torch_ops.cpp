@@ -369,7 +369,33 @@ void refuse_foreign_leaf(const at::Tensor& logits) {
               "evodiff_amd: an eager graph of these logits is alive: let go of its results before a pass with gradients is captured");
 }
 
+// The operators have no forward-mode derivative; a dual tensor does not ask for a gradient, and below autograd its tangent is lost.
+void refuse_tangent(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "evodiff_amd: ", name, " has no forward-mode derivative: give it the primal of a dual tensor");
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_autograd(const at::Tensor& x) {
+  refuse_tangent(x, "quantize_fp8");
+  const at::AutoDispatchBelowAutograd below;
+  return quantize_fp8(x);
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_weight_autograd(const at::Tensor& w) {
+  refuse_tangent(w, "quantize_fp8_weight");
+  const at::AutoDispatchBelowAutograd below;
+  return quantize_fp8_weight(w);
+}
+
+at::Tensor linear_fp8_autograd(const at::Tensor& x, const Maybe& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+                               const Maybe& bias, c10::optional<at::ScalarType> out_dtype, bool fast_sums) {
+  refuse_tangent(x, "linear_fp8");
+  if (bias.has_value()) refuse_tangent(*bias, "linear_fp8");
+  const at::AutoDispatchBelowAutograd below;
+  return linear_fp8(x, x_scale, weight, weight_scale, bias, out_dtype, fast_sums);
+}
+
 Scores token_logprobs_autograd(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
+  refuse_tangent(logits, "token_logprobs");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     const at::AutoDispatchBelowAutograd below;
     return token_logprobs(logits, targets, select, top_k, n_classes);
@@ -404,5 +430,8 @@ TORCH_LIBRARY_IMPL(evodiff_amd, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(evodiff_amd, AutogradCUDA, m) {
+  m.impl("quantize_fp8", &quantize_fp8_autograd);
+  m.impl("quantize_fp8_weight", &quantize_fp8_weight_autograd);
+  m.impl("linear_fp8", &linear_fp8_autograd);
   m.impl("token_logprobs", &token_logprobs_autograd);
 }

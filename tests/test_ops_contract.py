@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from evodiff_amd import _lib, ops
 from test_ops import (DTYPES, HALF, SHAPES, TILES, check_product, dequantized, dev, logprob_tolerance, plain_grad,  # noqa: F401
@@ -97,3 +98,37 @@ def test_fast_sums_of_the_c_entry_point():
         assert need >= 4096 * 32 * 129
         assert lib.ed_fp8_linear(p, 1, 4096, None, p, p, None, p, out, 4096, 4096, 4096, p, need - 1, None) == -1
         assert "workspace" in lib.ed_last_error().decode()
+
+
+# ---- derivatives -----------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused(dev, grad_mode):
+    """No operator has one, and none drops a tangent: the dual tensor is refused wherever it stands, in either grad mode."""
+    x, targets = rand(dev, (256, 256), 1), torch.zeros(256, dtype=torch.long, device=dev)
+    weight, rows, bias = ops.quantize_fp8_weight(x), ops.quantize_fp8(x), torch.zeros(256, device=dev)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual, dual_bias = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, bias))
+        for call in (lambda: ops.token_logprobs(dual, targets, 3), lambda: ops.token_logprobs(dual[:, 1:], None),
+                     lambda: ops.quantize_fp8(dual), lambda: ops.quantize_fp8_weight(dual), lambda: ops.linear_fp8(dual, weight),
+                     lambda: ops.linear_fp8(x, weight, dual_bias), lambda: ops.linear_fp8(rows, weight, dual_bias),
+                     lambda: ops.token_logprobs(forward_ad.make_dual(x.clone().requires_grad_(), x), targets)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        ops.token_logprobs(x, targets, 3)        # (beside dual tensors the others are as ever)
+        ops.linear_fp8(x, weight, bias)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda z: ops.token_logprobs(z, targets).logprob, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda z: ops.linear_fp8(z, weight), (x,), (x,))
+
+
+@gpu
+def test_transforms_give_the_operators_results_or_refuse(dev):
+    x, targets = rand(dev, (3, 5, 40), 1), torch.randint(0, 40, (3, 5), device=dev)
+    want = ops.token_logprobs(x, targets, 2)
+    got = torch.func.vmap(lambda z, t: tuple(ops.token_logprobs(z, t, 2)))(x, targets)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda z: ops.token_logprobs(z, targets).logprob.sum())(x)
