@@ -22,16 +22,31 @@ from . import torch_ops
 from ._lib import EvoDiffHipError
 
 
-class Fp8Rows(NamedTuple):
-    """Rows in 8 bits: ``q`` (rows, Kb * 128) float8_e4m3fn, ``scale`` (rows, Kb) float8_e8m0fnu, Kb = ceil(K / 128)."""
+class _Fp8Pair(NamedTuple):
     q: torch.Tensor
     scale: torch.Tensor
 
 
-class Fp8Weight(NamedTuple):
-    """A weight in 8 bits: ``q`` (N, Kb * 128) float8_e4m3fn, ``scale`` (ceil(N / 128), Kb) float8_e8m0fnu."""
-    q: torch.Tensor
-    scale: torch.Tensor
+class _Fp8Values(_Fp8Pair):
+    k: Optional[int] = None
+
+    def __new__(cls, q, scale, k=None):
+        pair = tuple.__new__(cls, (q, scale))
+        pair.k = k
+        return pair
+
+    def _replace(self, **fields):
+        return type(self)(*super()._replace(**fields), self.k)
+
+
+class Fp8Rows(_Fp8Values):
+    """Rows in 8 bits: a pair of ``q`` (rows, Kb * 128) float8_e4m3fn and ``scale`` (rows, Kb) float8_e8m0fnu, Kb = ceil(K / 128),
+    that remembers its width ``k`` = K (None for a pair made of two tensors alone: not known, and not checked)."""
+
+
+class Fp8Weight(_Fp8Values):
+    """A weight in 8 bits: a pair of ``q`` (N, Kb * 128) float8_e4m3fn and ``scale`` (ceil(N / 128), Kb) float8_e8m0fnu, with its
+    width ``k`` as in ``Fp8Rows``."""
 
 
 class TokenLogprobs(NamedTuple):
@@ -52,25 +67,27 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """``x`` (..., K) fp32 / bf16 / fp16 -> rows in 8 bits, a scale for 128 channels of a row (leading dimensions are
     flattened).  Rounded to nearest even; infinities and NaN become NaN."""
     _on_gpu(x)
-    return Fp8Rows(*torch_ops.load().quantize_fp8(x.detach() if x.requires_grad else x))
+    return Fp8Rows(*torch_ops.load().quantize_fp8(x.detach() if x.requires_grad else x), x.shape[-1])
 
 
 def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
     """``w`` (N, K) fp32 / bf16 / fp16 -> a weight in 8 bits, one scale for 128 x 128 values."""
     _on_gpu(w)
-    return Fp8Weight(*torch_ops.load().quantize_fp8_weight(w.detach() if w.requires_grad else w))
+    return Fp8Weight(*torch_ops.load().quantize_fp8_weight(w.detach() if w.requires_grad else w), w.shape[-1])
 
 
 def linear_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None, fast_sums: bool = False) -> torch.Tensor:
     """``x @ weight.T + bias`` with both operands in 8 bits and fp32 sums, rounded once.  ``x``: (..., K) fp32 / bf16 / fp16,
     quantised inside as ``quantize_fp8`` does (the results are equal bit for bit), or ``Fp8Rows`` for rows that several products
-    share.  ``weight``: from ``quantize_fp8_weight``.  ``bias``: fp32 (N,).  ``out_dtype``: that of ``x`` by default (bf16 for
+    share.  ``weight``: from ``quantize_fp8_weight``, of as many channels as ``x``.  ``bias``: fp32 (N,).  ``out_dtype``: that of ``x`` by default (bf16 for
     ``Fp8Rows``).  ``fast_sums`` (16-bit outputs): sums as the 8-bit matrix instruction takes them, up to three times as fast on large
     products - of eight neighbouring products the bits under 2^-13 of the largest are dropped (4e-5 to 6e-5 in 2-norm on ordinary
     data, up to 7 * 2^-13 of the terms' magnitudes, which is more than the rounding where large terms cancel).  An operator of inference: it has no gradient, and refuses an ``x`` or ``bias`` that asks for one."""
-    rows, scale = (x.q, x.scale) if isinstance(x, Fp8Rows) else (x, None)
+    rows, scale, k = (x.q, x.scale, x.k) if isinstance(x, Fp8Rows) else (x, None, x.shape[-1] if x.dim() else 0)
     _on_gpu(rows)
+    if k is not None and weight.k is not None and k != weight.k:
+        raise EvoDiffHipError("linear_fp8: x has %d channels, the weight has %d" % (k, weight.k))
     if torch.is_grad_enabled() and (rows.requires_grad or (bias is not None and bias.requires_grad)):
         raise EvoDiffHipError("linear_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
     if rows.requires_grad:

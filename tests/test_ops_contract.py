@@ -3,6 +3,7 @@ type, no derivative that is lost without a word, the widths of operands, rows th
 
 Tolerances are derived where they stand; a rounding is off by at most ``torch.finfo(t).eps / 2`` of the value.
 """
+import copy
 import ctypes
 import math
 
@@ -132,3 +133,31 @@ def test_transforms_give_the_operators_results_or_refuse(dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda z: ops.token_logprobs(z, targets).logprob.sum())(x)
+
+
+# ---- widths ----------------------------------------------------------------------------------------------------------
+
+def test_quantised_operands_are_pairs_that_know_their_width():
+    q, scale = torch.zeros((4, 256), dtype=torch.float8_e4m3fn), torch.zeros((1, 2), dtype=torch.float8_e8m0fnu)
+    for kind in (ops.Fp8Weight, ops.Fp8Rows):
+        one = kind(q, scale, 200)
+        a, b = one
+        assert a is q and b is scale and len(one) == 2 and one.q is q and one.scale is scale and one.k == 200
+        assert copy.copy(one).k == 200 and copy.deepcopy(one).k == 200 and one._replace(q=q).k == 200
+        assert kind(q, scale).k is None and kind(*one).k is None and kind(q=q, scale=scale, k=7).k == 7
+
+
+@gpu
+def test_linear_refuses_rows_of_another_width(dev):
+    x = rand(dev, (4, 1111), 1)
+    weight = ops.quantize_fp8_weight(rand(dev, (64, 1111), 0))
+    want = ops.linear_fp8(x, weight)
+    for other in (x[:, :1030], torch.nn.functional.pad(x, (0, 41)), x[:, :1110]):   # as many blocks of 128, another width
+        with pytest.raises(_lib.EvoDiffHipError, match="1111"):
+            ops.linear_fp8(other, weight)
+        with pytest.raises(_lib.EvoDiffHipError, match="1111"):
+            ops.linear_fp8(ops.quantize_fp8(other), weight)
+    assert ops.quantize_fp8(x).k == weight.k == 1111
+    assert torch.equal(ops.linear_fp8(ops.quantize_fp8(x), weight, out_dtype=torch.float32), want)
+    assert torch.equal(ops.linear_fp8(x, ops.Fp8Weight(weight.q, weight.scale)), want)          # width not known: not checked
+    assert torch.equal(ops.linear_fp8(ops.Fp8Rows(*ops.quantize_fp8(x)), weight, out_dtype=torch.float32), want)
