@@ -374,22 +374,28 @@ void refuse_tangent(const at::Tensor& t, const char* name) {
   TORCH_CHECK(!t._fw_grad(0).defined(), "evodiff_amd: ", name, " has no forward-mode derivative: give it the primal of a dual tensor");
 }
 
+// What has no derivative at all says so where one is asked for.
+void refuse_derivatives(const at::Tensor& t, const char* name) {
+  refuse_tangent(t, name);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !t.requires_grad(), "evodiff_amd: ", name, " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_autograd(const at::Tensor& x) {
-  refuse_tangent(x, "quantize_fp8");
+  refuse_derivatives(x, "quantize_fp8");
   const at::AutoDispatchBelowAutograd below;
   return quantize_fp8(x);
 }
 
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_weight_autograd(const at::Tensor& w) {
-  refuse_tangent(w, "quantize_fp8_weight");
+  refuse_derivatives(w, "quantize_fp8_weight");
   const at::AutoDispatchBelowAutograd below;
   return quantize_fp8_weight(w);
 }
 
 at::Tensor linear_fp8_autograd(const at::Tensor& x, const Maybe& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
                                const Maybe& bias, c10::optional<at::ScalarType> out_dtype, bool fast_sums) {
-  refuse_tangent(x, "linear_fp8");
-  if (bias.has_value()) refuse_tangent(*bias, "linear_fp8");
+  refuse_derivatives(x, "linear_fp8");
+  if (bias.has_value()) refuse_derivatives(*bias, "linear_fp8");
   const at::AutoDispatchBelowAutograd below;
   return linear_fp8(x, x_scale, weight, weight_scale, bias, out_dtype, fast_sums);
 }

@@ -11,7 +11,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from evodiff_amd import _lib, ops
+from evodiff_amd import _lib, ops, torch_ops
 from test_ops import (DTYPES, HALF, SHAPES, TILES, check_product, dequantized, dev, logprob_tolerance, plain_grad,  # noqa: F401
                       plain_logprobs, plain_quantize, rand, rel_ok)
 
@@ -161,3 +161,24 @@ def test_linear_refuses_rows_of_another_width(dev):
     assert torch.equal(ops.linear_fp8(ops.quantize_fp8(x), weight, out_dtype=torch.float32), want)
     assert torch.equal(ops.linear_fp8(x, ops.Fp8Weight(weight.q, weight.scale)), want)          # width not known: not checked
     assert torch.equal(ops.linear_fp8(ops.Fp8Rows(*ops.quantize_fp8(x)), weight, out_dtype=torch.float32), want)
+
+
+@gpu
+def test_quantisation_does_not_drop_a_gradient(dev):
+    x = rand(dev, (4, 256), 1).requires_grad_()
+    for quantize in (ops.quantize_fp8, ops.quantize_fp8_weight):
+        with pytest.raises(_lib.EvoDiffHipError, match="no gradient"):
+            quantize(x)
+        with pytest.raises(_lib.EvoDiffHipError, match="no gradient"):
+            quantize(x * 2)
+        want = quantize(x.detach())
+        with torch.no_grad():
+            got = quantize(x)
+        assert torch.equal(got.q.float(), want.q.float()) and not got.q.requires_grad
+    for name in ("quantize_fp8", "quantize_fp8_weight"):     # the operators underneath as well
+        with pytest.raises(RuntimeError, match="no gradient"):
+            getattr(torch_ops.load(), name)(x)
+    weight = ops.quantize_fp8_weight(x.detach())
+    for args in ((x, None, *weight, None, None), (x.detach(), None, *weight, torch.zeros(4, device=dev, requires_grad=True), None)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            torch_ops.load().linear_fp8(*args)
