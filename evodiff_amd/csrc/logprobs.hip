@@ -714,7 +714,8 @@ __device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* 
   a.h = g.entropy[r];
   a.weight = g.g_logprob ? g.g_logprob[r] : 0.f;
   a.g_h = g.g_entropy ? g.g_entropy[r] : 0.f;
-  if (targets && (targets[r] < 0 || targets[r] >= x.n)) a.weight = __builtin_nanf("");
+  // (a target that is no class: its log probability is NaN, and so is a gradient that comes through it; no other does)
+  if (a.weight != 0.f && targets && (targets[r] < 0 || targets[r] >= x.n)) a.weight = __builtin_nanf("");
   return a;
 }
 // what the named classes of row r add to class v

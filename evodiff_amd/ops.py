@@ -110,7 +110,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top_k:
     ``targets``: int64, shaped like the logits without classes, or None.  ``select``: bool or uint8 of that shape; rows where it is
     false are not read: results 0, tokens -1, gradient 0.  ``n_classes``: only the first ``n_classes`` classes count.
     -inf forbids a class; a row without any other has logprob -inf, entropy 0, alternatives at -inf and no gradient.  A row with
-    NaN or +inf yields NaN, and so does a target outside [0, n_classes) for its logprob.  Logits may be a view with up to two
+    NaN or +inf yields NaN, and so does a target outside [0, n_classes) for its logprob, and for the row's gradient if that logprob
+    has a part in the loss.  Logits may be a view with up to two
     strided leading dimensions (``logits[:, :-1]``); others are copied first.
 
     Differentiable once in ``logprob``, ``entropy`` and ``top_logprob``."""

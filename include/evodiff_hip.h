@@ -305,7 +305,8 @@ int ed_fp8_linear(const void* x_dev, int x_dtype, int64_t row_stride, const uint
  * evenly spaced rows.  fp32 sums whatever the type.
  *   -inf forbids a class (log probability -inf).  A row without any other class: logprob -inf, entropy 0, top
  *   alternatives 0, 1, ... at -inf, gradient 0.  A row with NaN or +inf: logprob, entropy and top_logprob NaN, tokens
- *   some class, gradient NaN.  A target outside [0, n_classes): logprob and gradient NaN, nothing is read there.
+ *   some class, gradient NaN.  A target outside [0, n_classes): logprob NaN, nothing is read there; the
+ *   row's gradient is NaN if its grad_logprob is not 0, and does not depend on the target if it is.
  *   select_dev (rows bytes, may be NULL = every row): a row with a zero byte is not read; its results are 0, its tokens -1,
  *   its gradient 0.
  * targets_dev may be NULL: logprob_dev is then not written (and may be NULL).  logprob_dev, entropy_dev fp32 [rows];

@@ -182,3 +182,40 @@ def test_quantisation_does_not_drop_a_gradient(dev):
     for args in ((x, None, *weight, None, None), (x.detach(), None, *weight, torch.zeros(4, device=dev, requires_grad=True), None)):
         with pytest.raises(RuntimeError, match="no gradient"):
             torch_ops.load().linear_fp8(*args)
+
+
+# ---- gradient --------------------------------------------------------------------------------------------------------
+
+def gradient_tolerance(x, v, g_lp, g_h, g_top, want, dtype):
+    """As in test_gradient: p is off by the tolerance of a log probability and multiplies terms of these sizes; then a rounding."""
+    size = g_lp.abs() + g_top.abs().sum(1) + g_h.abs() * 64
+    tol = 4 * logprob_tolerance(x.detach().float().cpu(), v) * size[:, None].double()
+    return tol + (want.abs() + tol) * HALF[dtype] + torch.finfo(dtype).smallest_normal * HALF[dtype] * 2
+
+
+@gpu
+@pytest.mark.parametrize("v", [31, 700, 20001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_where_a_target_is_none(dev, v, dtype):
+    """A target outside the classes makes its log probability NaN; what does not depend on it stays as it is, and so does a gradient
+    to which that log probability contributes nothing."""
+    rows = 6
+    x = rand(dev, (rows, v), v, dtype).requires_grad_()
+    targets = torch.tensor([-100, 3, v, 0, -1, 1 << 40])
+    valid = (targets >= 0) & (targets < v)
+    out = ops.token_logprobs(x, targets.to(dev), 4)
+    assert torch.isnan(out.logprob.cpu()).tolist() == (~valid).tolist()
+    g_h, g_top = torch.linspace(-1, 1, rows), torch.linspace(1, 2, rows * 4).view(rows, 4)
+    token, zero = out.top_token.cpu(), torch.zeros(rows)
+    # entropy and alternatives alone
+    grad, = torch.autograd.grad(out[1:3], x, (g_h.to(dev), g_top.to(dev)), retain_graph=True)
+    want = plain_grad(x, None, token, None, zero.double(), g_h.double(), g_top.double())
+    assert float(((grad.cpu().double() - want).abs() - gradient_tolerance(x, v, zero, g_h, g_top, want, dtype)).max()) <= 0
+    # a loss that leaves the rows without a target out of its sum
+    kept = torch.where(valid.to(dev), out.logprob, torch.zeros_like(out.logprob))
+    grad, = torch.autograd.grad((kept.sum(),) + out[1:3], x, (torch.ones((), device=dev), g_h.to(dev), g_top.to(dev)), retain_graph=True)
+    want = plain_grad(x, targets.clamp(0, v - 1), token, None, valid.double(), g_h.double(), g_top.double())
+    assert float(((grad.cpu().double() - want).abs() - gradient_tolerance(x, v, valid.float(), g_h, g_top, want, dtype)).max()) <= 0
+    # one that takes them in
+    grad, = torch.autograd.grad(out.logprob.sum(), x)
+    assert torch.isnan(grad.cpu()).all(1).tolist() == (~valid).tolist()
