@@ -702,7 +702,9 @@ struct GradRow {
   bool skip;
   __device__ __forceinline__ float at(float x) const {
     const float lp = (x - m) - log_s, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    return -p * fmaf(g_h, max_nan(lp, -1.0e30f) + h, weight);  // (a forbidden class: nothing, not nothing times infinity)
+    // From log p = -200 on p is 0, far under the least value of the type; held there, the other factor stays finite for incoming
+    // gradients up to 1e36: a forbidden class gets nothing, not nothing times infinity.
+    return -p * fmaf(g_h, max_nan(lp, -200.0f) + h, weight);
   }
 };
 __device__ __forceinline__ GradRow grad_row(const LogitsView& x, const int64_t* targets, const uint8_t* select,

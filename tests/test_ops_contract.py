@@ -219,3 +219,19 @@ def test_gradient_where_a_target_is_none(dev, v, dtype):
     # one that takes them in
     grad, = torch.autograd.grad(out.logprob.sum(), x)
     assert torch.isnan(grad.cpu()).all(1).tolist() == (~valid).tolist()
+
+
+@gpu
+@pytest.mark.parametrize("v", [31, 700, 20001])
+@pytest.mark.parametrize("scale", [1e9, -1e30])
+def test_gradient_of_a_scaled_entropy_is_zero_at_forbidden_classes(dev, v, scale):
+    x = rand(dev, (4, v), v)
+    x[0, 1::3], x[1, ::2], x[2, 1:] = -math.inf, torch.finfo(torch.float32).min, -1e6
+    x[3, 5:] = -150.0
+    x.requires_grad_()
+    g_h, zero = torch.full((4,), scale), torch.zeros(4)
+    grad, = torch.autograd.grad(ops.token_logprobs(x, None).entropy, x, g_h.to(dev))
+    want = plain_grad(x, None, torch.zeros((4, 0), dtype=torch.long), None, zero.double(), g_h.double(), torch.zeros((4, 0)).double())
+    off = (grad.cpu().double() - want).abs() - gradient_tolerance(x, v, zero, g_h, torch.zeros((4, 0)), want, torch.float32)
+    assert float(off.max()) <= 0, float(off.max())
+    assert bool((grad[0, 1::3] == 0).all()) and bool((grad[1, ::2] == 0).all()) and bool((grad[2, 1:] == 0).all())
