@@ -361,11 +361,10 @@ void refuse_foreign_leaf(const at::Tensor& logits) {
   if (!logits.is_leaf()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(logits);
   if (!node) return;
-  const c10::Stream now = c10::hip::getCurrentHIPStream(logits.device().index()).unwrap();
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   TORCH_CHECK(hipStreamIsCapturing((hipStream_t)current_stream(logits), &status) == hipSuccess, "evodiff_amd: hipStreamIsCapturing failed");
-  const auto made = node->stream();
-  TORCH_CHECK(status == hipStreamCaptureStatusNone || !made.has_value() || *made == now,
+  const auto made = node->stream();  // (its device's type is not that of a HIP stream: by number)
+  TORCH_CHECK(status == hipStreamCaptureStatusNone || !made.has_value() || made->id() == c10::hip::getCurrentHIPStream(logits.device().index()).id(),
               "evodiff_amd: an eager graph of these logits is alive: let go of its results before a pass with gradients is captured");
 }
 

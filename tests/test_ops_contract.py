@@ -235,3 +235,32 @@ def test_gradient_of_a_scaled_entropy_is_zero_at_forbidden_classes(dev, v, scale
     off = (grad.cpu().double() - want).abs() - gradient_tolerance(x, v, zero, g_h, torch.zeros((4, 0)), want, torch.float32)
     assert float(off.max()) <= 0, float(off.max())
     assert bool((grad[0, 1::3] == 0).all()) and bool((grad[1, ::2] == 0).all()) and bool((grad[2, 1:] == 0).all())
+
+
+# ---- capture ---------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("passes", [1, 3])
+def test_capture_of_a_leaf_that_is_used_more_than_once(dev, passes):
+    """The accumulation node of a leaf that is first used inside the capture belongs to its stream: later uses there are no foreign ones."""
+    logits = rand(dev, (40, 700), 3).requires_grad_()
+    targets, ones = torch.randint(0, 700, (2, 40), device=dev), torch.ones(40, device=dev)
+
+    def step():
+        grads = []
+        for _ in range(passes):
+            outs = [ops.token_logprobs(logits, t, 3) for t in targets]
+            grads += torch.autograd.grad([outs[0].logprob, outs[1].logprob, outs[1].entropy], logits, [ones, ones, ones])
+        return grads
+
+    want = step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for _ in range(3):
+        for t in captured:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
