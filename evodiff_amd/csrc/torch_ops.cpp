@@ -357,9 +357,11 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 // A leaf's accumulation node belongs to the stream of the graph that made it and lives as long as that graph.  A backward pass
 // that is captured on another stream would make that stream wait inside the capture, which the engine's thread does not survive.
+// The logits are the leaf, or a view of it.
 void refuse_foreign_leaf(const at::Tensor& logits) {
-  if (!logits.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(logits);
+  const at::TensorBase& leaf = logits.is_view() ? logits._base() : logits;
+  if (!leaf.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
   if (!node) return;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   TORCH_CHECK(hipStreamIsCapturing((hipStream_t)current_stream(logits), &status) == hipSuccess, "evodiff_amd: hipStreamIsCapturing failed");

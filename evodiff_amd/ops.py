@@ -9,8 +9,8 @@ They run on PyTorch's current stream of the tensors' device, through ``torch.ops
 C ABI (``ed_token_logprobs``, ``ed_fp8_*`` in include/evodiff_hip.h).  There is no CPU path.  Outputs and workspaces come from
 PyTorch's allocator, so the calls can be captured into a HIP graph.  A backward pass is captured together with its forward and
 asks for its gradients with ``torch.autograd.grad``: ``.backward()`` accumulates into leaves on the stream that first used
-them.  While an eager graph of the same leaf logits is alive, a forward with gradients refuses to be captured.  None of them has a forward-mode derivative: dual
-tensors are refused.
+them.  While an eager graph of the same leaf logits, or of the leaf that they are a view of, is alive, a forward with gradients
+refuses to be captured.  None of them has a forward-mode derivative: dual tensors are refused.
 """
 from __future__ import annotations
 

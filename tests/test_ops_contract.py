@@ -5,6 +5,7 @@ Tolerances are derived where they stand; a rounding is off by at most ``torch.fi
 """
 import copy
 import ctypes
+import gc
 import math
 
 import pytest
@@ -264,3 +265,41 @@ def test_capture_of_a_leaf_that_is_used_more_than_once(dev, passes):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+VIEWS = {"columns": lambda z: z[:, 1:], "rows": lambda z: z[::2], "view of a view": lambda z: z.view(4, 10, 700)[:, :-1, :650],
+         "expanded": lambda z: z[:1].expand(5, 700), "turned": lambda z: z.view(20, 2, 700).transpose(0, 1)}
+
+
+@gpu
+@pytest.mark.parametrize("view", VIEWS)
+def test_capture_with_an_eager_graph_of_the_leaf_under_a_view(dev, view):
+    """Refused while that graph is alive (only the forward is tried); captured, replayed and right once it is gone."""
+    leaf = rand(dev, (40, 700), 3).requires_grad_()
+    shape = VIEWS[view](leaf.detach()).shape
+    targets, ones = torch.randint(0, 600, shape[:-1], device=dev), torch.ones(shape[:-1], device=dev)
+
+    def forward():
+        return ops.token_logprobs(VIEWS[view](leaf), targets, 3)
+
+    def step():
+        out = forward()
+        return torch.autograd.grad((out.logprob, out.entropy), leaf, (ones, ones))[0]
+
+    want = step()
+    alive = forward()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            forward()
+    assert torch.equal(torch.autograd.grad((alive.logprob, alive.entropy), leaf, (ones, ones))[0], want)
+    del alive
+    gc.collect()                                  # (the refusal's traceback held the view that it was raised for)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for _ in range(3):
+        captured.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+        assert torch.equal(step(), want)
