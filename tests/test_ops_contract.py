@@ -303,3 +303,130 @@ def test_capture_with_an_eager_graph_of_the_leaf_under_a_view(dev, view):
         torch.cuda.synchronize()
         assert torch.equal(captured, want)
         assert torch.equal(step(), want)
+
+
+# ---- forms of the kernels that ordinary cases seldom take ------------------------------------------------------------
+
+def shifted(x):
+    """64 bits, each row less its largest value: the operators are functions of differences, and a sum of exponentials beside a value of
+    1e38 is lost in 64 bits too."""
+    x = x.detach().cpu().double()
+    largest = x.amax(1, keepdim=True)
+    return x - torch.where(torch.isfinite(largest), largest, torch.zeros_like(largest))
+
+
+def graded(view, targets, k, n_classes, select=None, seed=1):
+    """The gradient of a view's three results to the tensor under it, and the formula's."""
+    v, shape = view.shape[-1], view.shape[:-1]
+    rows = math.prod(shape)
+    g = torch.Generator().manual_seed(seed)
+    g_lp, g_h, g_top = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.randn((rows, k), generator=g)
+    out = ops.token_logprobs(view, targets, k, select, n_classes)
+    parts = [(out.entropy, g_h.view(shape)), (out.top_logprob, g_top.view(shape + (k,)))]
+    if targets is None:
+        g_lp = torch.zeros(rows)
+    else:
+        parts.append((out.logprob, g_lp.view(shape)))
+    grad, = torch.autograd.grad([p for p, _ in parts], view, [q.to(view.device) for _, q in parts])
+    flat = view.detach().reshape(rows, v)
+    want = plain_grad(shifted(flat), None if targets is None else targets.reshape(-1).cpu(), out.top_token.reshape(rows, k).cpu().clamp(min=0),
+                      None if select is None else select.reshape(-1).cpu(), g_lp.double(), g_h.double(), g_top.double(), n_classes)
+    off = (grad.reshape(rows, v).cpu().double() - want).abs()
+    assert float((off - gradient_tolerance(flat, v, g_lp, g_h, g_top, want, view.dtype)).max()) <= 0
+    if n_classes is not None:
+        assert bool((grad[..., n_classes:] == 0).all())
+    return grad
+
+
+@gpu
+@pytest.mark.parametrize("columns", [257, 1001, 1008, 4099, 40003])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_many_columns_at_every_alignment(dev, columns, dtype):
+    """Sources that start on another alignment than the gradient's rows, one and two strides, classes and alternatives on the
+    borders of vectors, tiles and pieces."""
+    base = rand(dev, (3, 4, columns + 8), columns, dtype)
+    n = columns
+    for at in (0, 1, 3, 7):
+        for view in (base[:, 0, at:at + n], base[:, :-1, at:at + n], base[1, :, at:at + n]):
+            view = view.detach().requires_grad_()
+            assert view.stride(-1) == 1 and not view.is_contiguous()
+            rows = math.prod(view.shape[:-1])
+            border = torch.tensor([0, 1, 7, 8, 255, 256, 2047, 2048, 2049, 4095, 4096, 8191, 16383, 16384, n - 9, n - 8, n - 2, n - 1])
+            border = border[(border >= 0) & (border < n)]
+            targets = border[torch.arange(rows) * 5 % len(border)].view(view.shape[:-1]).to(dev)
+            graded(view, targets, 6, None, seed=at)
+            graded(view, None, 2, None, seed=at)
+
+
+@gpu
+@pytest.mark.parametrize("n_classes", [1, 3, 7, 8, 9, 300, 992, 1000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_is_zero_behind_few_classes_of_many_columns(dev, n_classes, dtype):
+    x = rand(dev, (5, 1001), 3, dtype)
+    x[:, n_classes:] = math.nan                       # behind the classes nothing is read
+    for view in (x, x[:4].view(2, 2, 1001), torch.nn.functional.pad(x, (1, 6))[:, 1:1002]):
+        view = view.detach().requires_grad_()
+        targets = (torch.arange(math.prod(view.shape[:-1])) * 7 % n_classes).view(view.shape[:-1]).to(dev)
+        graded(view, targets, min(n_classes, 5), n_classes)
+
+
+@gpu
+@pytest.mark.parametrize("rows,v", [(7, 257), (9, 4099), (40, 20000), (300, 3000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_rows_left_out(dev, rows, v, dtype):
+    """Rows that are left out, whatever stands in them, and rows without a class: zeros, and their neighbours as without them."""
+    x = rand(dev, (rows, v), v, dtype)
+    left, empty = torch.arange(rows) % 3 == 1, torch.arange(rows) % 5 == 3
+    x[left.to(dev)] = math.nan
+    x[empty.to(dev)] = -math.inf
+    view = x.detach().requires_grad_()
+    targets = torch.arange(rows, device=dev) * 13 % v
+    grad = graded(view, targets, 4, None, select=~left.to(dev))
+    assert bool((grad[(left | empty).to(dev)] == 0).all())
+
+
+def check_rows(dev, x, targets, k):
+    got, want = ops.token_logprobs(x, targets.to(dev), k), plain_logprobs(shifted(x), targets, k)
+    tol = logprob_tolerance(torch.zeros(1), x.shape[1])
+    assert torch.equal(got.top_token.cpu(), want[3])
+    for a, b, t in ((got.logprob, want[0], tol), (got.entropy, want[1], 2 * tol), (got.top_logprob, want[2], tol)):
+        rel_ok(a, torch.where(b.abs() > torch.finfo(torch.float32).max, b * math.inf, b), t)     # (as the result's type has it)
+    if x.shape[0] * x.shape[1] < 1 << 21:
+        graded(x.detach().requires_grad_(), targets.to(dev), k, None)
+
+
+@gpu
+@pytest.mark.parametrize("rows,v,k", [(3, 4096, 20), (5, 4093, 32), (2100, 4800, 20), (600, 40000, 20), (1, 1 << 20, 20), (2, 700001, 7)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_of_rising_rows(dev, rows, v, k, dtype):
+    """More groups reach the bound than the list holds: a wave a row, a workgroup a row, pieces of a row."""
+    x = (torch.arange(v, dtype=torch.float64) * (40.0 / v) - 20.0).to(dtype).to(dev).expand(rows, v)
+    x = x.contiguous() if rows < 100 else x          # (many equal rows under one stride of 0)
+    got = ops.token_logprobs(x, torch.arange(rows, device=dev), k)
+    few = min(rows, 2)
+    want = plain_logprobs(x[:few], torch.arange(few), k)
+    tol = logprob_tolerance(x[:1].float().cpu(), v)
+    assert torch.equal(got.top_token[:few].cpu(), want[3]) and bool((got.top_token == got.top_token[0]).all())
+    rel_ok(got.logprob[:few], want[0], tol)
+    rel_ok(got.entropy[:few], want[1], 2 * tol)
+    rel_ok(got.top_logprob[:few], want[2], tol)
+
+
+@gpu
+@pytest.mark.parametrize("rows,v,k", [(8, 3000, 5), (8, 600, 20), (600, 9000, 3), (8, 40000, 20), (8, 31, 5), (8, 500, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_any_magnitude(dev, rows, v, k, dtype):
+    """Largest values past +-2^20, where base 2 is too coarse, up to the type's own, every class at its lowest, and a spread that
+    passes the type's range: a row's results depend on differences alone."""
+    x = torch.randint(0, 8, (rows, v), generator=torch.Generator().manual_seed(v)).float()
+    top = torch.finfo(dtype).max
+    x[0] = 2.0e6 - x[0] * 8192
+    x[1] = -2.0e6 - x[1] * 8192
+    x[2] = 1048568.0 + x[2]                           # (under 2^20: the largest in base 2)
+    x[3] = torch.where(x[3] == 0, 1.0e30, -1.0e30)
+    x[4] = torch.where(x[4] < 4, -1.0e30, -2.0e30)
+    x[5] = -top
+    x[6] = torch.where(x[6] == 3, top, -top)
+    x[7] = torch.where(x[7] == 5, -top, -math.inf)
+    targets = (torch.arange(rows) * 11) % v
+    check_rows(dev, x.to(dtype).to(dev), targets, k)
