@@ -761,6 +761,21 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
     const int vectors = x.n > head ? (x.n - head) / EPV : 0;
     const int v0 = piece * per * 256 < vectors ? piece * per * 256 : vectors;
     const int v1 = v0 + per * 256 < vectors && piece + 1 < pieces ? v0 + per * 256 : vectors;
+    auto edges = [&](auto one) {  // one(column) for those of this piece that no vector holds
+      if (vectors > 0) {
+        if (piece == 0 && tid < head) one(tid);
+        if (piece + 1 == pieces)
+          for (long v = head + (long)vectors * EPV + tid; v < g.columns; v += 256) one(v);
+      } else {
+        const long span = (g.columns + pieces - 1) / pieces, to = (piece + 1) * span < g.columns ? (piece + 1) * span : g.columns;
+        for (long v = piece * span + tid; v < to; v += 256) one(v);
+      }
+    };
+    if (select && !select[r]) {  // left out: nothing of the row is read (4096 x 32000 bf16 with half of them 70 -> 55 us)
+      for (int vec = v0 + tid; vec < v1; vec += 256) __builtin_nontemporal_store(VT{}, (VT*)(dst + head + (long)vec * EPV));
+      edges([&](long v) { dst[v] = Elem<DT>::put(0.f); });
+      continue;
+    }
     uint4 next[U];
     auto load = [&](int at) {
 #pragma unroll
@@ -828,7 +843,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
         __builtin_nontemporal_store(o, (VT*)(dst + first));
       }
     }
-    auto one = [&](long v) {
+    edges([&](long v) {
       float d = 0.f;
       if (!a.skip && v < x.n) {
         d = a.at(Elem<DT>::get(row[v]));
@@ -839,15 +854,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitsView x, const 
           }
       }
       dst[v] = Elem<DT>::put(d);
-    };
-    if (vectors > 0) {
-      if (piece == 0 && tid < head) one(tid);
-      if (piece + 1 == pieces)
-        for (long v = head + (long)vectors * EPV + tid; v < g.columns; v += 256) one(v);
-    } else {
-      const long span = (g.columns + pieces - 1) / pieces, to = (piece + 1) * span < g.columns ? (piece + 1) * span : g.columns;
-      for (long v = piece * span + tid; v < to; v += 256) one(v);
-    }
+    });
   }
 }
 
