@@ -29,7 +29,7 @@ template <>
 struct Elem<DT_FP16> { typedef _Float16 T; };
 
 // Vectors that are aligned to their element alone: the memory instructions take any address, so that odd widths and strides move 16
-// bytes at a time as others do (4452 x 3354 x 2092 fp16 53 us, value by value 85).
+// bytes at a time as others do (4452 x 3354 x 2092 fp16, 8-bit sums, 53 us, value by value 85).
 template <typename T, int N>
 struct Loose {
   typedef __attribute__((ext_vector_type(N))) T V;
@@ -184,9 +184,11 @@ __device__ __forceinline__ int load_byte(buffer_t src, unsigned lane_off, unsign
 // taps, then blocks; a tap moves the row operand by `dilation` rows of its padded layout, whose rows around a sequence hold
 // zeros.  Taps that move a whole tile outside its sequence are left out.
 //
-// Measured, TFLOP/s with the launch: 8192^3 390 us, 2820 (a library's product on the same values 402 us: the matrix pipe under that
-// chip's clock); 16384 x 1280 x 1280 32 us, 1670 (ten steps of K: a third of the time is the tile's start and its
-// stores); a convolution of five taps, 1280 channels and 16384 positions 121 us, 2200 counting all taps, exact 8192^3 1350 us, 815.
+// Measured on rows in 8 bits, ten calls in a captured graph, a call with its scales turned: 8-bit sums 8192^3 386 us, 2850 TFLOP/s (a
+// library's product on the same values 402 us: the matrix pipe under that chip's clock), 16384 x 1280 x 1280 33 us, 1630 (ten steps
+// of K: a third of the time is the tile's start and its stores); EXACT 1266 us, 870, and 73 us, 730: bound by its vector
+// instructions, some 16 to widen (shared by a wave's tile) and a dozen to scale and add for four matrix ones.  Under a kernel trace
+// the large products take a tenth longer.  A convolution of five taps, 1280 channels and 16384 positions 121 us, 2200 counting all taps.
 template <int WM, int WTM, int WTN, int S, int OUT_DT, bool EXACT, bool TAPS>
 __global__ __launch_bounds__(128 * WM, WM / 2) void tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n) {
   constexpr int WAVES = 2 * WM, BM = 16 * WM * WTM, BN = 32 * WTN, STAGE = (BM + BN) * 128;
@@ -465,8 +467,9 @@ __global__ __launch_bounds__(128 * WM, WM / 2) void tile_kernel(Fp8Gemm g, int t
 // 16 rows and 16 NF channels, its waves share the blocks of K (wave w: w, w + waves, ...): a wave reads a block's weights as fragments straight from memory, the next
 // block's in flight, and brings plain rows to 8 bits in registers - the four lanes that hold a row's block find its
 // largest magnitude with two exchanges.  The waves' sums meet in shared memory, in order.
-// Measured: 8 x 8192 x 8192 17.2 us, 67 MB of weights at 3.9 TB/s (a copy: 4.7; the start and the join of a single round of
-// workgroups are the rest); 1 x 1280 x 1280 4.5 us, where a launch alone takes 2 to 3.
+// Measured, calls in a captured graph, exact (8-bit sums): 8 x 8192 x 8192 on rows in 8 bits 18.2 us (17.7), 67 MB of weights at 3.7 TB/s (a
+// copy: 4.7; the start and the join of a single round of workgroups are the rest); 1 x 1280 x 1280 5.0 us (4.7), where a launch
+// alone takes 2 to 3.
 // ---------------------------------------------------------------------------------------------------
 // 32 values of a row: columns k0 .. k0 + 15 and k0 + 64 .. k0 + 79, zeros behind K
 template <int DT>
@@ -681,8 +684,10 @@ struct Plan {
 // The cheapest by what was measured of the tiles (microseconds).  A step of K takes a tile no less than `step` alone on its CU (its
 // latency), all tiles at work together no less than their copies take at 16 GB/ms of L2 and their products at `rate`; a round of
 // tiles has 2 to 3 us of start and end, and its results to write.  A cut K loop adds a launch and its sums' way through
-// memory.  Sides measured: 16384 x 1280 x 1280 tiles of 256 x 320 34 us, 256 x 256 47, 128 x 128 41; 4096^3 67, 55 and 69; 512 x 8192 x 8192 128-tiles
-// 46, 64-tiles 59; 1024 x 1280 x 1280 12.1 and 11.2; 128 x 8192 x 8192 64-tiles whole 28.6, K cut in two 25.5.
+// memory.  Sides measured with 8-bit sums: 16384 x 1280 x 1280 tiles of 256 x 320 34 us, 256 x 256 47, 128 x 128 41; 4096^3 67, 55 and 69; 512 x 8192 x 8192 128-tiles
+// 46, 64-tiles 59; 1024 x 1280 x 1280 12.1 and 11.2; 128 x 8192 x 8192 64-tiles whole 28.6, K cut in two 25.5 - there the cost errs: it
+// says 19.0 and 26.5, and takes the first.  What the exact form takes and the cost says: 32 x 8192 x 8192 27.5 (20), 128 rows 44 (34), 512
+// rows 133 (102), 16384 x 1280 x 1280 73 (88), 8192^3 1266 (1510).
 static Plan plan_of(int64_t M, int64_t N, int kb, bool exact, bool whole_k = false) {
   struct Kind {
     int size, bm, bn, resident;
@@ -736,15 +741,15 @@ static hipError_t launch_plan(const Fp8Gemm& g, const Plan& p, hipStream_t strea
 }
 
 // The few-rows kernel takes up to 16 rows always, and more where 16 x 16 outputs by 128 channels make no more than FEW_WORK pieces
-// and a wave no more than four steps: one launch, no wait between the steps of K.  Sides measured (us, rows already in 8 bits, bf16
-// and fp32 outputs; the tiles need the scales turned first): 64 x 1280 x 1280 6.8 and 6.4, tiles 10.6 and 13.3; 300 x 1111 x 1000
+// and a wave no more than four steps: one launch, no wait between the steps of K.  Sides measured (us, rows already in 8 bits, 8-bit
+// and exact sums; the tiles need the scales turned first): 64 x 1280 x 1280 6.8 and 6.4, tiles 10.6 and 13.3; 300 x 1111 x 1000
 // (10640 pieces) 8.4 and 9.1, tiles 10.6 and 13.4; plain rows there 11.2 and 11.7, tiles 10.6 and 13.8; 1024 x 640 x 640 (12800) 12.4
-// and 13.1, tiles 10.3 and 10.4.
+// and 13.1, tiles 10.3 and 10.4.  One limit for both sums, by the exact ones (plain rows with 8-bit sums would turn a little sooner).
 constexpr int FEW_ROWS = 16, FEW_WORK = 11000, FEW_K = 64;
 static int64_t few_work(int64_t M, int64_t N, int64_t kb) { return ((M + 15) / 16) * ((N + 15) / 16) * kb; }
 static bool few_rows(int64_t M, int64_t N, int64_t kb) { return M <= FEW_ROWS || (kb <= FEW_K && few_work(M, N, kb) <= FEW_WORK); }
 // Plain rows are brought to 8 bits inside that kernel (every workgroup does it again) up to this many blocks of K (8 x 2560 x 2560
-// 7.6 us against 10.3 with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3) and, beyond 16 rows, pieces (bf16 and fp32: 4096 x
+// 7.6 us against 10.3 with a launch of its own, 4 x 5120 x 5120 16.6 against 12.3) and, beyond 16 rows, pieces (8-bit and exact sums: 4096 x
 // 31 x 1280, 5120 pieces, 6.6 and 6.7 against 10.0 and 10.4; 128 x 640 x 2560, 6400 pieces, 7.8 and 10.3 against 10.2 and 10.4;
 // 300 x 1111 x 1000, 10640 pieces, 10.0 and 11.2 against 10.4 and 11.0).
 constexpr int FEW_BLOCKS = 24, FEW_INSIDE = 8000;
