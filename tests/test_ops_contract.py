@@ -430,3 +430,25 @@ def test_rows_of_any_magnitude(dev, rows, v, k, dtype):
     x[7] = torch.where(x[7] == 5, -top, -math.inf)
     targets = (torch.arange(rows) * 11) % v
     check_rows(dev, x.to(dtype).to(dev), targets, k)
+
+
+@gpu
+@pytest.mark.parametrize("v", [2, 12, 31, 33, 64, 200, 256, 300, 512])
+@pytest.mark.parametrize("gap", [0.0, 2.0, 6.0, 12.0, 30.0])
+def test_log_probability_of_a_class_that_is_all_but_certain(dev, v, gap):
+    """Few classes: exact relative to its own size, and the entropy likewise.  With the others' sum r of terms p = exp(-d), log S =
+    log1p(r).  A term is off by the rounding of d, that of d log2(e) and the constant's own (2.3 d 2^-24 together, d at most the row's
+    spread) and by two roundings of the exponential, the sum of n terms in chains of 16 and 6 by 22, log1p by two; T the same and a
+    product: (2.5 d + 30) 2^-24 of each.  The entropy is a sum of two such positive values and their quotient."""
+    x = rand(dev, (300, v), v)
+    at, targets = torch.arange(300, device=dev), torch.arange(300, device=dev) % v
+    x[at, targets] = x.amax(1) + gap
+    got = ops.token_logprobs(x, targets, 1)
+    d = x.double() - x[at, targets].double()[:, None]
+    others = torch.exp(d).scatter(1, targets[:, None], 0.0)
+    log_s = torch.log1p(others.sum(1))
+    entropy = log_s - (d * others).sum(1) / (1 + others.sum(1))
+    tol = (2.5 * float(-d.min()) + 30) * 2.0 ** -24
+    assert float(((got.logprob.double() + log_s).abs() / log_s).max()) <= tol
+    assert float(((got.top_logprob[:, 0].double() + log_s).abs() / log_s).max()) <= tol
+    assert float(((got.entropy.double() - entropy).abs() / entropy).max()) <= 2 * tol
