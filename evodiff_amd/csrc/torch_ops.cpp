@@ -381,31 +381,40 @@ void refuse_derivatives(const at::Tensor& t, const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !t.requires_grad(), "evodiff_amd: ", name, " has no gradient: call it under torch.no_grad() or on detached tensors");
 }
 
+// The operator again, below autograd: through the dispatcher, so that dispatch modes and tensors without data (fake ones) are met
+// there and not in the kernel's own code.
+template <typename Signature>
+auto operator_of(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>(); }
+
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_autograd(const at::Tensor& x) {
   refuse_derivatives(x, "quantize_fp8");
+  static const auto op = operator_of<decltype(quantize_fp8)>("evodiff_amd::quantize_fp8");
   const at::AutoDispatchBelowAutograd below;
-  return quantize_fp8(x);
+  return op.call(x);
 }
 
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_weight_autograd(const at::Tensor& w) {
   refuse_derivatives(w, "quantize_fp8_weight");
+  static const auto op = operator_of<decltype(quantize_fp8_weight)>("evodiff_amd::quantize_fp8_weight");
   const at::AutoDispatchBelowAutograd below;
-  return quantize_fp8_weight(w);
+  return op.call(w);
 }
 
 at::Tensor linear_fp8_autograd(const at::Tensor& x, const Maybe& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
                                const Maybe& bias, c10::optional<at::ScalarType> out_dtype, bool fast_sums) {
   refuse_derivatives(x, "linear_fp8");
   if (bias.has_value()) refuse_derivatives(*bias, "linear_fp8");
+  static const auto op = operator_of<decltype(linear_fp8)>("evodiff_amd::linear_fp8");
   const at::AutoDispatchBelowAutograd below;
-  return linear_fp8(x, x_scale, weight, weight_scale, bias, out_dtype, fast_sums);
+  return op.call(x, x_scale, weight, weight_scale, bias, out_dtype, fast_sums);
 }
 
 Scores token_logprobs_autograd(const at::Tensor& logits, const Maybe& targets, const Maybe& select, int64_t top_k, int64_t n_classes) {
   refuse_tangent(logits, "token_logprobs");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    static const auto op = operator_of<decltype(token_logprobs)>("evodiff_amd::token_logprobs");
     const at::AutoDispatchBelowAutograd below;
-    return token_logprobs(logits, targets, select, top_k, n_classes);
+    return op.call(logits, targets, select, top_k, n_classes);
   }
   refuse_foreign_leaf(logits);
   const auto out = TokenLogprobs::apply(logits, targets, select, top_k, n_classes);

@@ -10,7 +10,9 @@ import math
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from evodiff_amd import _lib, ops, torch_ops
 from test_ops import (DTYPES, HALF, SHAPES, TILES, check_product, dequantized, dev, logprob_tolerance, plain_grad,  # noqa: F401
@@ -452,3 +454,33 @@ def test_log_probability_of_a_class_that_is_all_but_certain(dev, v, gap):
     assert float(((got.logprob.double() + log_s).abs() / log_s).max()) <= tol
     assert float(((got.top_logprob[:, 0].double() + log_s).abs() / log_s).max()) <= tol
     assert float(((got.entropy.double() - entropy).abs() / entropy).max()) <= 2 * tol
+
+
+# ---- dispatch --------------------------------------------------------------------------------------------------------
+
+def test_tensors_without_data_are_refused_by_the_dispatcher():
+    """Fake tensors (no GPU is needed for them) never reach a kernel: the operators have no form for them."""
+    with FakeTensorMode():
+        x = torch.empty((4, 256), device="cuda")
+        weight = ops.Fp8Weight(torch.empty((64, 256), dtype=torch.float8_e4m3fn, device="cuda"),
+                               torch.empty((1, 2), dtype=torch.float8_e8m0fnu, device="cuda"))
+        for call in (lambda: ops.quantize_fp8(x), lambda: ops.quantize_fp8_weight(x), lambda: ops.linear_fp8(x, weight),
+                     lambda: ops.token_logprobs(x, torch.empty(4, dtype=torch.long, device="cuda"))):
+            with pytest.raises(RuntimeError, match="evodiff_amd"):
+                call()
+
+
+@gpu
+def test_dispatch_modes_see_the_operators(dev):
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    x, names = rand(dev, (4, 256), 1), []
+    want = ops.linear_fp8(ops.quantize_fp8(x), ops.quantize_fp8_weight(x))
+    with Seen():
+        got = ops.linear_fp8(ops.quantize_fp8(x), ops.quantize_fp8_weight(x))
+        ops.token_logprobs(x, None, 2)
+    assert torch.equal(got, want)
+    assert [n.split("::")[1] for n in names if n.startswith("evodiff_amd::")] == ["quantize_fp8", "quantize_fp8_weight", "linear_fp8", "token_logprobs"]
