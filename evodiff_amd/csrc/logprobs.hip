@@ -122,8 +122,8 @@ __device__ __forceinline__ void skip_row(const LogprobsOut& out, long r, int top
 
 // ---------------------------------------------------------------------------------------------------
 // Few classes (n <= G * E <= 512): G lanes own a row and keep it in registers, lane j the classes j, j + G, ...  The alternatives are
-// taken one after the other, a largest key of the group each.  64 x 31 fp32 top 5 and 16384 x 31 both 4 us on the GPU, most of
-// it the launch: bound by the host's call (8.8 us).
+// taken one after the other, a largest key of the group each.  64 x 31 fp32 top 5 4.5 us on the GPU, 16384 x 31
+// without alternatives 3.5, most of it the launch: bound by the host's call (9.0 us).
 // ---------------------------------------------------------------------------------------------------
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
